@@ -7,7 +7,7 @@ Importing the package on a machine without the built library raises
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint16, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint16, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libffnrm.so"
@@ -16,6 +16,8 @@ OK, ERR_ARG, ERR_CUDA, ERR_STATE, ERR_NOMEM, ERR_TIMEOUT = 0, 1, 2, 3, 4, 5
 CODES_Q4_BYTES, CODES_QLO2_ROWPACKED, CODES_BITPLANES = 0, 1, 2
 KERNEL_RESIDUAL, KERNEL_DOWN, KERNEL_REDUCE = 0, 1, 2
 IPC_HANDLE_BYTES = 64
+F16, BF16, F32 = 0, 1, 2
+ROTARY_INTERLEAVED, ROTARY_INVERSE = 1, 2
 
 # Every symbol include/ffnrm.h declares, with its ctypes signature.
 SIGNATURES = {
@@ -53,6 +55,20 @@ SIGNATURES = {
     "ffnrm_base_from_table": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int,
                                       c_void_p, c_int64, c_void_p]),
     "ffnrm_table_dots": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "ffnrm_rotary": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+                             c_void_p]),
+    "ffnrm_kv_create": (c_int, [POINTER(c_void_p), c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ffnrm_kv_destroy": (c_int, [c_void_p]),
+    "ffnrm_kv_append": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                c_void_p, c_int, c_int, c_int, c_void_p]),
+    "ffnrm_kv_read": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "ffnrm_kv_attend": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_float, c_int,
+                                c_int, c_void_p]),
+    "ffnrm_kv_fork": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                              c_void_p, c_void_p, c_void_p]),
+    "ffnrm_kv_compact": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "ffnrm_kv_copy_pages": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "ffnrm_kv_check": (c_int, [c_void_p, c_void_p]),
     "ffnrm_last_error": (c_char_p, []),
     "ffnrm_version": (c_char_p, []),
 }
@@ -68,6 +84,20 @@ class LayerWeights(ctypes.Structure):
                 ("gate_high", c_void_p), ("up_high", c_void_p), ("gate_alpha", c_void_p), ("up_alpha", c_void_p),
                 ("gate_beta", c_void_p), ("up_beta", c_void_p), ("down", c_void_p), ("down_ld", c_int64),
                 ("keep_fallback", c_int32)]
+
+
+class KvConfig(ctypes.Structure):
+    _fields_ = [("n_layers", c_int32), ("n_pages", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("page_tokens", c_int32), ("max_seqs", c_int32)]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("tables", c_void_p), ("lengths", c_void_p), ("starts", c_void_p), ("seqs", c_int32),
+                ("table_width", c_int32), ("rows", c_int32)]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("token_stride", c_int64), ("head_stride", c_int64)]
 
 
 class NativeLibraryMissing(RuntimeError):

@@ -8,9 +8,11 @@ statically, so it needs only the driver at run time.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -18,7 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libffnrm.so"
-SOURCES = [CSRC / "ffnrm.cu", PKG / "host" / "base_producer.cpp"]
+SOURCES = [CSRC / "ffnrm.cu", CSRC / "kv.cu", PKG / "host" / "base_producer.cpp"]
 HEADERS = sorted(CSRC.glob("*.cuh")) + sorted((PKG / "host").glob("*.hpp")) + [ROOT / "include" / "ffnrm.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -30,10 +32,35 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def command(out: Path = LIB, extra: list[str] | None = None) -> list[str]:
-    return [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "--shared", "-Xcompiler", "-fPIC",
-            "-cudart", "static", "-Xcompiler", "-mavx2", "-I", str(ROOT / "include"), "-I", str(CSRC), "-I", str(PKG / "host"),
-            *(extra or []), *map(str, SOURCES), "-o", str(out)]
+INCLUDES = ["-I", str(ROOT / "include"), "-I", str(CSRC), "-I", str(PKG / "host")]
+
+
+def object_path(source: Path) -> Path:
+    return LIB_DIR / (source.name + ".o")
+
+
+def compile_command(source: Path) -> list[str]:
+    return [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-c", "-Xcompiler", "-fPIC", "-Xcompiler", "-mavx2",
+            *INCLUDES, str(source), "-o", str(object_path(source))]
+
+
+def link_command(out: Path = LIB) -> list[str]:
+    return [nvcc(), *ARCH, "--shared", "-Xcompiler", "-fPIC", "-cudart", "static", *(str(object_path(s)) for s in SOURCES),
+            "-o", str(out)]
+
+
+def included(source: Path) -> list[Path]:
+    """The source and every in-tree header it reaches through quoted includes."""
+    found, todo = [], [source]
+    while todo:
+        path = todo.pop()
+        found.append(path)
+        for name in re.findall(r'^#include "([^"]+)"', path.read_text(), flags=re.M):
+            for folder in (path.parent, ROOT / "include", CSRC, PKG / "host"):
+                if (folder / name).exists() and folder / name not in found + todo:
+                    todo.append(folder / name)
+                    break
+    return found
 
 
 # Drop-in runner executables (same argv / exit codes / JSON as the reference's runners),
@@ -74,10 +101,14 @@ def build_runners(force: bool = False, verbose: bool = False) -> list[Path]:
 def build(force: bool = False, verbose: bool = False, runners: bool = True) -> Path:
     if force or stale():
         LIB_DIR.mkdir(exist_ok=True)
-        cmd = command()
+        todo = [compile_command(s) for s in SOURCES if force or stale(object_path(s), included(s))]
         if verbose:
-            print(" ".join(cmd), file=sys.stderr)
-        subprocess.run(cmd, check=True)
+            for cmd in [*todo, link_command()]:
+                print(" ".join(cmd), file=sys.stderr)
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            for done in pool.map(subprocess.run, todo):
+                done.check_returncode()
+        subprocess.run(link_command(), check=True)
     if runners:
         build_runners(force, verbose)
     return LIB

@@ -45,6 +45,15 @@ int fail(int code, const char *fmt, ...) {
     return code;
 }
 
+}  // namespace
+
+// The library's other translation units report through the same per-thread message.
+namespace ffnrm {
+int set_error(int code, const char *message) { return fail(code, "%s", message); }
+}  // namespace ffnrm
+
+namespace {
+
 #define FFNRM_CUDA(expr)                                                                          \
     do {                                                                                          \
         cudaError_t _e = (expr);                                                                  \

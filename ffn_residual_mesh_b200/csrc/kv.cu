@@ -1,0 +1,442 @@
+// C ABI of the 8-bit paged cache and its operators (include/ffnrm.h, ffnrm_rotary, ffnrm_kv_*).
+#include "ffnrm.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <new>
+
+#include "kv_append.cuh"
+#include "kv_attend.cuh"
+#include "kv_common.cuh"
+#include "kv_pages.cuh"
+#include "kv_rotary.cuh"
+
+namespace ffnrm {
+int set_error(int code, const char *message);  // ffnrm.cu
+}
+
+namespace {
+
+using namespace ffnrm::kv;
+
+int fail(int code, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return ffnrm::set_error(code, buf);
+}
+
+#define KV_CUDA(expr)                                                                                        \
+    do {                                                                                                     \
+        cudaError_t _e = (expr);                                                                             \
+        if (_e != cudaSuccess)                                                                               \
+            return fail(FFNRM_ERR_CUDA, "%s failed at %s:%d: %s", #expr, __FILE__, __LINE__, cudaGetErrorString(_e)); \
+    } while (0)
+
+struct DeviceGuard {
+    int prev = -1;
+    explicit DeviceGuard(int dev) {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != dev) cudaSetDevice(dev);
+    }
+    ~DeviceGuard() {
+        int cur = -1;
+        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+    }
+};
+
+bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+size_t type_size(int dtype) { return dtype == FFNRM_F32 ? 4 : 2; }
+
+// Whether a row block can be read in 16-byte accesses.
+bool wide(const ffnrm_rows &r, int dtype) {
+    const int64_t n = 16 / int64_t(type_size(dtype));
+    return aligned(r.data, 16) && r.token_stride % n == 0 && r.head_stride % n == 0;
+}
+
+int check_rows(const char *name, const ffnrm_rows *r, int dtype) {
+    if (!r || !r->data) return fail(FFNRM_ERR_ARG, "%s: null rows", name);
+    if (!aligned(r->data, type_size(dtype))) return fail(FFNRM_ERR_ARG, "%s: misaligned rows", name);
+    return FFNRM_OK;
+}
+
+int check_table(const float *table, int rotary_dim, int max_positions, int head_dim, int flags, int allowed) {
+    if (!table || !aligned(table, 4)) return fail(FFNRM_ERR_ARG, "null or misaligned rotary table");
+    if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > head_dim)
+        return fail(FFNRM_ERR_ARG, "rotary_dim=%d must be even, positive and at most head_dim=%d", rotary_dim, head_dim);
+    if (max_positions <= 0) return fail(FFNRM_ERR_ARG, "max_positions=%d must be positive", max_positions);
+    if (flags & ~allowed) return fail(FFNRM_ERR_ARG, "unknown rotary flags %d", flags);
+    return FFNRM_OK;
+}
+
+template <typename T, bool INTERLEAVED>
+void launch_rotary(const RotaryArgs &a, float sign, bool vec, cudaStream_t st) {
+    constexpr int N = 16 / int(sizeof(T));
+    const bool wide_rows = vec && rotary_fits<INTERLEAVED, N>(a.dim, a.rot);
+    const int units = wide_rows ? rotary_units<INTERLEAVED, N>(a.dim, a.rot) : rotary_units<INTERLEAVED, 1>(a.dim, a.rot);
+    const int64_t n = int64_t(a.tokens) * a.heads * units;
+    const unsigned grid = unsigned(std::min<int64_t>((n + 255) / 256, 1 << 20));
+    if (wide_rows)
+        rotary_kernel<T, INTERLEAVED, N><<<grid, 256, 0, st>>>(a, sign);
+    else
+        rotary_kernel<T, INTERLEAVED, 1><<<grid, 256, 0, st>>>(a, sign);
+}
+
+}  // namespace
+
+struct ffnrm_kv {
+    int device = 0;
+    ffnrm_kv_config cfg{};
+    int page_shift = 0;
+    int8_t *k_codes = nullptr, *v_codes = nullptr;
+    float *k_scale = nullptr, *v_scale = nullptr;
+    int num_sms = 148;
+    int *status = nullptr;       // what kernels could not use, kStatus* bits
+    int32_t *scratch = nullptr;  // page lists of fork / compact
+    int32_t *src = nullptr, *dst = nullptr, *owner = nullptr, *list = nullptr, *rows = nullptr, *count = nullptr;
+};
+
+namespace {
+
+int check_kv(ffnrm_kv *kv, int layer) {
+    if (!kv) return fail(FFNRM_ERR_ARG, "null cache");
+    if (layer < 0 || layer >= kv->cfg.n_layers)
+        return fail(FFNRM_ERR_ARG, "layer %d out of range [0, %d)", layer, kv->cfg.n_layers);
+    return FFNRM_OK;
+}
+
+int check_batch(ffnrm_kv *kv, const ffnrm_kv_batch *b) {
+    if (!b) return fail(FFNRM_ERR_ARG, "null batch");
+    if (b->seqs < 0 || b->seqs > kv->cfg.max_seqs)
+        return fail(FFNRM_ERR_ARG, "seqs=%d outside [0, max_seqs=%d]", b->seqs, kv->cfg.max_seqs);
+    if (b->rows < 0 || b->table_width < 0) return fail(FFNRM_ERR_ARG, "rows and table_width must not be negative");
+    if ((int64_t(b->table_width) << kv->page_shift) > (int64_t(1) << 30))
+        return fail(FFNRM_ERR_ARG, "table_width=%d addresses more than 2^30 tokens", b->table_width);
+    if (!b->starts && b->rows != b->seqs)
+        return fail(FFNRM_ERR_ARG, "without starts there is one row per sequence: rows=%d, seqs=%d", b->rows, b->seqs);
+    if (b->seqs > 0 && (!b->lengths || (b->table_width > 0 && !b->tables)))
+        return fail(FFNRM_ERR_ARG, "null tables or lengths");
+    if (!aligned(b->tables, 4) || !aligned(b->lengths, 4) || !aligned(b->starts, 4))
+        return fail(FFNRM_ERR_ARG, "tables, lengths and starts must be 4-byte aligned");
+    return FFNRM_OK;
+}
+
+Pool layer_pool(const ffnrm_kv *kv, int layer) {
+    const ffnrm_kv_config &c = kv->cfg;
+    const int64_t ph = int64_t(layer) * c.n_pages * c.kv_heads, codes = ph * c.page_tokens * c.head_dim;
+    return Pool{kv->k_codes + codes, kv->v_codes + codes, kv->k_scale + ph, kv->v_scale + ph,
+                c.n_pages,           c.kv_heads,          c.head_dim,       c.page_tokens,    kv->page_shift};
+}
+
+Batch batch_view(const ffnrm_kv_batch *b) { return Batch{b->tables, b->lengths, b->starts, b->seqs, b->table_width, b->rows}; }
+
+template <typename T>
+void launch_append(const AppendArgs &a, bool vec, bool interleaved, unsigned grid, cudaStream_t st) {
+    if (vec && interleaved)
+        append_kernel<T, true, true><<<grid, 256, 0, st>>>(a);
+    else if (vec)
+        append_kernel<T, true, false><<<grid, 256, 0, st>>>(a);
+    else if (interleaved)
+        append_kernel<T, false, true><<<grid, 256, 0, st>>>(a);
+    else
+        append_kernel<T, false, false><<<grid, 256, 0, st>>>(a);
+}
+
+template <typename T>
+void launch_attend(const AttendArgs &a, unsigned grid, cudaStream_t st) {
+    if (a.pool.dim == 64)
+        attend_rows_kernel<T, 64><<<grid, 128, 0, st>>>(a);
+    else if (a.pool.dim == 128)
+        attend_rows_kernel<T, 128><<<grid, 128, 0, st>>>(a);
+    else
+        attend_rows_kernel<T, 256><<<grid, 128, 0, st>>>(a);
+}
+
+int launch_moves(ffnrm_kv *kv, const int32_t *src, const int32_t *dst, const int32_t *count, int most, cudaStream_t st) {
+    const ffnrm_kv_config &c = kv->cfg;
+    const int page_bytes = c.kv_heads * c.page_tokens * c.head_dim;
+    MoveArgs m{kv->k_codes, kv->v_codes, kv->k_scale, kv->v_scale, src,  dst,       count,
+               c.n_layers,  c.n_pages,   c.kv_heads,  page_bytes,  most, kv->status};
+    const int64_t items = int64_t(most) * c.n_layers * 2 * ((page_bytes + kMoveChunk - 1) / kMoveChunk);
+    const unsigned grid = unsigned(std::min<int64_t>(items, int64_t(kv->num_sms) * 8));
+    move_kernel<<<grid, 256, 0, st>>>(m);
+    KV_CUDA(cudaGetLastError());
+    return FFNRM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ffnrm_rotary(const ffnrm_rows *x, const ffnrm_rows *y, int dtype, int tokens, int heads, int head_dim,
+                 const int32_t *positions, const float *table, int rotary_dim, int max_positions, int flags,
+                 void *stream) {
+    if (dtype < FFNRM_F16 || dtype > FFNRM_F32) return fail(FFNRM_ERR_ARG, "unknown element type %d", dtype);
+    if (tokens < 0 || heads < 0 || head_dim <= 0)
+        return fail(FFNRM_ERR_ARG, "tokens=%d, heads=%d, head_dim=%d are no shape", tokens, heads, head_dim);
+    int rc = check_table(table, rotary_dim, max_positions, head_dim, flags, FFNRM_ROTARY_INTERLEAVED | FFNRM_ROTARY_INVERSE);
+    if (rc) return rc;
+    if (tokens == 0 || heads == 0) return FFNRM_OK;
+    if ((rc = check_rows("x", x, dtype)) || (rc = check_rows("y", y, dtype))) return rc;
+    if (!positions || !aligned(positions, 4)) return fail(FFNRM_ERR_ARG, "null or misaligned positions");
+    if (x->data == y->data && (x->token_stride != y->token_stride || x->head_stride != y->head_stride))
+        return fail(FFNRM_ERR_ARG, "rotating in place needs equal strides");
+    const RotaryArgs a{x->data, y->data, positions, table, x->token_stride, x->head_stride, y->token_stride, y->head_stride,
+                       tokens, heads, head_dim, rotary_dim, max_positions};
+    const bool vec = wide(*x, dtype) && wide(*y, dtype), inter = flags & FFNRM_ROTARY_INTERLEAVED;
+    const float sign = flags & FFNRM_ROTARY_INVERSE ? -1.f : 1.f;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FFNRM_F16)
+        inter ? launch_rotary<__half, true>(a, sign, vec, st) : launch_rotary<__half, false>(a, sign, vec, st);
+    else if (dtype == FFNRM_BF16)
+        inter ? launch_rotary<__nv_bfloat16, true>(a, sign, vec, st) : launch_rotary<__nv_bfloat16, false>(a, sign, vec, st);
+    else
+        inter ? launch_rotary<float, true>(a, sign, vec, st) : launch_rotary<float, false>(a, sign, vec, st);
+    KV_CUDA(cudaGetLastError());
+    return FFNRM_OK;
+}
+
+int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8_t *k_codes, int8_t *v_codes,
+                    float *k_scale, float *v_scale) {
+    if (!out || !cfg) return fail(FFNRM_ERR_ARG, "null argument");
+    *out = nullptr;
+    const ffnrm_kv_config &c = *cfg;
+    if (c.n_layers <= 0 || c.kv_heads <= 0 || c.kv_heads > 1024)
+        return fail(FFNRM_ERR_ARG, "n_layers=%d must be positive, kv_heads=%d in [1, 1024]", c.n_layers, c.kv_heads);
+    if (c.n_pages <= 0 || c.n_pages > (1 << 20)) return fail(FFNRM_ERR_ARG, "n_pages=%d outside [1, 1048576]", c.n_pages);
+    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
+        return fail(FFNRM_ERR_ARG, "head_dim=%d must be 64, 128 or 256", c.head_dim);
+    if (c.page_tokens != 16 && c.page_tokens != 32 && c.page_tokens != 64 && c.page_tokens != 128)
+        return fail(FFNRM_ERR_ARG, "page_tokens=%d must be 16, 32, 64 or 128", c.page_tokens);
+    if (c.max_seqs <= 0 || c.max_seqs > 4096) return fail(FFNRM_ERR_ARG, "max_seqs=%d outside [1, 4096]", c.max_seqs);
+    if (!k_codes || !v_codes || !k_scale || !v_scale) return fail(FFNRM_ERR_ARG, "null pool");
+    if (!aligned(k_codes, 16) || !aligned(v_codes, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
+        return fail(FFNRM_ERR_ARG, "code pools must be 16-byte aligned, scale pools 4-byte");
+    ffnrm_kv *kv = new (std::nothrow) ffnrm_kv;
+    if (!kv) return fail(FFNRM_ERR_NOMEM, "out of host memory");
+    kv->device = device;
+    kv->cfg = c;
+    while ((1 << kv->page_shift) < c.page_tokens) ++kv->page_shift;
+    kv->k_codes = k_codes;
+    kv->v_codes = v_codes;
+    kv->k_scale = k_scale;
+    kv->v_scale = v_scale;
+    int count = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count) {
+        cudaGetLastError();
+        delete kv;
+        return fail(FFNRM_ERR_CUDA, "no CUDA device %d", device);
+    }
+    DeviceGuard guard(device);
+    cudaDeviceGetAttribute(&kv->num_sms, cudaDevAttrMultiProcessorCount, device);
+    const size_t list = size_t(std::max(c.n_pages, c.max_seqs));
+    const size_t ints = 4 * list + 4 * size_t(c.max_seqs) + 2;
+    const int bitmap = (c.n_pages + 31) / 32 * 4;
+    if (cudaMalloc(&kv->scratch, ints * sizeof(int32_t)) != cudaSuccess) {
+        cudaGetLastError();
+        delete kv;
+        return fail(FFNRM_ERR_NOMEM, "cudaMalloc of %zu bytes failed", ints * sizeof(int32_t));
+    }
+    kv->src = kv->scratch;
+    kv->dst = kv->src + list;
+    kv->owner = kv->dst + list;
+    kv->list = kv->owner + list;
+    kv->rows = kv->list + list;
+    kv->count = kv->rows + 4 * size_t(c.max_seqs);
+    kv->status = kv->count + 1;
+    cudaError_t e = cudaMemset(kv->scratch, 0, ints * sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(bitmap, 1 << 17));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(bitmap, 1 << 17));
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) {
+        cudaFree(kv->scratch);
+        delete kv;
+        return fail(FFNRM_ERR_CUDA, "creating the cache failed: %s", cudaGetErrorString(e));
+    }
+    *out = kv;
+    return FFNRM_OK;
+}
+
+int ffnrm_kv_destroy(ffnrm_kv *kv) {
+    if (!kv) return FFNRM_OK;
+    DeviceGuard guard(kv->device);
+    cudaFree(kv->scratch);  // waits for the device
+    cudaGetLastError();
+    delete kv;
+    return FFNRM_OK;
+}
+
+int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, const ffnrm_rows *k,
+                    const ffnrm_rows *v, const ffnrm_rows *q, const ffnrm_rows *q_out, int q_heads, const float *table,
+                    int rotary_dim, int max_positions, int flags, void *stream) {
+    int rc = check_kv(kv, layer);
+    if (rc || (rc = check_batch(kv, batch))) return rc;
+    if (dtype < FFNRM_F16 || dtype > FFNRM_F32) return fail(FFNRM_ERR_ARG, "unknown element type %d", dtype);
+    const int D = kv->cfg.head_dim;
+    if (table && (rc = check_table(table, rotary_dim, max_positions, D, flags, FFNRM_ROTARY_INTERLEAVED))) return rc;
+    const bool has_q = q && q->data;
+    if (has_q && !table) return fail(FFNRM_ERR_ARG, "q is only rotated: it needs a rotary table");
+    if (has_q && q_heads <= 0) return fail(FFNRM_ERR_ARG, "q_heads=%d must be positive", q_heads);
+    if (batch->rows == 0 || batch->seqs == 0) return FFNRM_OK;
+    if ((rc = check_rows("k", k, dtype)) || (rc = check_rows("v", v, dtype))) return rc;
+    if (has_q) {
+        if ((rc = check_rows("q_out", q_out, dtype)) || (rc = check_rows("q", q, dtype))) return rc;
+        if (q->data == q_out->data && (q->token_stride != q_out->token_stride || q->head_stride != q_out->head_stride))
+            return fail(FFNRM_ERR_ARG, "rotating in place needs equal strides");
+    }
+    const bool inter = flags & FFNRM_ROTARY_INTERLEAVED;
+    const int N = 16 / int(type_size(dtype));
+    bool vec = wide(*k, dtype) && wide(*v, dtype) && (!has_q || (wide(*q, dtype) && wide(*q_out, dtype)));
+    if (has_q) vec = vec && rotary_dim % N == 0 && (inter || (rotary_dim / 2) % N == 0);
+    AppendArgs a{};
+    a.pool = layer_pool(kv, layer);
+    a.batch = batch_view(batch);
+    a.k = k->data, a.k_token = k->token_stride, a.k_head = k->head_stride;
+    a.v = v->data, a.v_token = v->token_stride, a.v_head = v->head_stride;
+    a.table = table, a.rot = table ? rotary_dim : 0, a.max_positions = max_positions;
+    a.slots = append_slots(batch->seqs, batch->rows, kv->page_shift, batch->starts != nullptr);
+    a.status = kv->status;
+    int64_t grid = int64_t(a.slots) * kv->cfg.kv_heads * 2;
+    if (has_q) {
+        a.q = q->data, a.q_token = q->token_stride, a.q_head = q->head_stride;
+        a.q_out = q_out->data, a.o_token = q_out->token_stride, a.o_head = q_out->head_stride;
+        a.q_heads = q_heads;
+        const int units = vec ? (inter ? rotary_units<true, 1>(D, 0) / N : (rotary_dim / 2 + D - rotary_dim) / N)
+                              : rotary_units<false, 1>(D, rotary_dim);
+        a.q_chunks = (units * q_heads + 255) / 256;
+        grid += int64_t(batch->rows) * a.q_chunks;
+    }
+    if (grid > 0x7fffffff) return fail(FFNRM_ERR_ARG, "rows=%d are too many for one call", batch->rows);
+    DeviceGuard guard(kv->device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FFNRM_F16)
+        launch_append<__half>(a, vec, inter, unsigned(grid), st);
+    else if (dtype == FFNRM_BF16)
+        launch_append<__nv_bfloat16>(a, vec, inter, unsigned(grid), st);
+    else
+        launch_append<float>(a, vec, inter, unsigned(grid), st);
+    KV_CUDA(cudaGetLastError());
+    return FFNRM_OK;
+}
+
+int ffnrm_kv_read(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, void *k, void *v, void *stream) {
+    int rc = check_kv(kv, layer);
+    if (rc || (rc = check_batch(kv, batch))) return rc;
+    if (dtype < FFNRM_F16 || dtype > FFNRM_F32) return fail(FFNRM_ERR_ARG, "unknown element type %d", dtype);
+    if (batch->rows == 0 || batch->seqs == 0) return FFNRM_OK;
+    if (!k || !v || !aligned(k, 16) || !aligned(v, 16)) return fail(FFNRM_ERR_ARG, "k and v must be 16-byte aligned");
+    const ReadArgs a{layer_pool(kv, layer), batch_view(batch), k, v, kv->status};
+    DeviceGuard guard(kv->device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FFNRM_F16)
+        read_kernel<__half><<<unsigned(batch->rows), 256, 0, st>>>(a);
+    else if (dtype == FFNRM_BF16)
+        read_kernel<__nv_bfloat16><<<unsigned(batch->rows), 256, 0, st>>>(a);
+    else
+        read_kernel<float><<<unsigned(batch->rows), 256, 0, st>>>(a);
+    KV_CUDA(cudaGetLastError());
+    return FFNRM_OK;
+}
+
+int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, const ffnrm_rows *q,
+                    const ffnrm_rows *out, float *lse, int q_heads, float scale, int causal, int window, void *stream) {
+    int rc = check_kv(kv, layer);
+    if (rc || (rc = check_batch(kv, batch))) return rc;
+    if (dtype != FFNRM_F16 && dtype != FFNRM_BF16) return fail(FFNRM_ERR_ARG, "q and out are f16 or bf16, got type %d", dtype);
+    if (q_heads <= 0 || q_heads % kv->cfg.kv_heads)
+        return fail(FFNRM_ERR_ARG, "q_heads=%d must be a multiple of kv_heads=%d", q_heads, kv->cfg.kv_heads);
+    if (window < 0) return fail(FFNRM_ERR_ARG, "window=%d must not be negative", window);
+    if (!(scale == scale) || scale <= 0.f || scale > 3.4e38f) return fail(FFNRM_ERR_ARG, "scale must be positive and finite");
+    if (batch->rows == 0) return FFNRM_OK;
+    if (batch->seqs == 0) return fail(FFNRM_ERR_ARG, "rows=%d of no sequence", batch->rows);
+    if ((rc = check_rows("q", q, dtype)) || (rc = check_rows("out", out, dtype))) return rc;
+    if (!wide(*q, dtype) || !wide(*out, dtype))
+        return fail(FFNRM_ERR_ARG, "q and out rows must be 16-byte aligned");
+    if (!aligned(lse, 4)) return fail(FFNRM_ERR_ARG, "lse must be 4-byte aligned");
+    const AttendArgs a{layer_pool(kv, layer), batch_view(batch), q->data, out->data, lse, q->token_stride, q->head_stride,
+                       out->token_stride, out->head_stride, q_heads / kv->cfg.kv_heads, scale, causal, window, kv->status};
+    const int64_t grid = (int64_t(batch->rows) * q_heads + 3) / 4;
+    if (grid > 0x7fffffff) return fail(FFNRM_ERR_ARG, "rows=%d are too many for one call", batch->rows);
+    DeviceGuard guard(kv->device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == FFNRM_F16)
+        launch_attend<__half>(a, unsigned(grid), st);
+    else
+        launch_attend<__nv_bfloat16>(a, unsigned(grid), st);
+    KV_CUDA(cudaGetLastError());
+    return FFNRM_OK;
+}
+
+int ffnrm_kv_fork(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, int seqs, int table_width,
+                  const int32_t *parents, const int32_t *extra, int children, int32_t *out_tables, int out_width,
+                  int32_t *out_lengths, int32_t *info, void *stream) {
+    if (!kv) return fail(FFNRM_ERR_ARG, "null cache");
+    if (seqs < 0 || seqs > kv->cfg.max_seqs || children < 0 || children > kv->cfg.max_seqs)
+        return fail(FFNRM_ERR_ARG, "seqs=%d and children=%d must lie in [0, max_seqs=%d]", seqs, children, kv->cfg.max_seqs);
+    if (table_width < 0 || out_width < 0 || (int64_t(std::max(table_width, out_width)) << kv->page_shift) > (int64_t(1) << 30))
+        return fail(FFNRM_ERR_ARG, "table widths %d and %d must address at most 2^30 tokens", table_width, out_width);
+    if (!info || (children && (!parents || !extra || !out_lengths || (out_width && !out_tables))) ||
+        (seqs && (!lengths || (table_width && !tables))))
+        return fail(FFNRM_ERR_ARG, "null device pointer");
+    if (out_tables && out_tables == tables) return fail(FFNRM_ERR_ARG, "out_tables must not be the input tables");
+    DeviceGuard guard(kv->device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const PageArgs a{tables, lengths, parents, extra, out_tables, out_lengths, info, kv->src, kv->dst, kv->count, kv->owner,
+                     kv->list, kv->rows, seqs, table_width, children, out_width, kv->cfg.n_pages, kv->page_shift, kv->status};
+    fork_kernel<<<1, kPageThreads, size_t(kv->cfg.n_pages + 31) / 32 * 4, st>>>(a);
+    KV_CUDA(cudaGetLastError());
+    if (children == 0) return FFNRM_OK;
+    return launch_moves(kv, kv->src, kv->dst, kv->count, std::min(children, kv->cfg.n_pages), st);
+}
+
+int ffnrm_kv_compact(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, int seqs, int table_width,
+                     int32_t *out_tables, int32_t *info, void *stream) {
+    if (!kv) return fail(FFNRM_ERR_ARG, "null cache");
+    if (seqs < 0 || seqs > kv->cfg.max_seqs) return fail(FFNRM_ERR_ARG, "seqs=%d outside [0, max_seqs=%d]", seqs, kv->cfg.max_seqs);
+    if (table_width < 0 || (int64_t(table_width) << kv->page_shift) > (int64_t(1) << 30))
+        return fail(FFNRM_ERR_ARG, "table_width=%d must address at most 2^30 tokens", table_width);
+    if (!info || (seqs && (!lengths || (table_width && (!tables || !out_tables)))))
+        return fail(FFNRM_ERR_ARG, "null device pointer");
+    DeviceGuard guard(kv->device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const PageArgs a{tables, lengths, nullptr, nullptr, out_tables, nullptr, info, kv->src, kv->dst, kv->count, kv->owner,
+                     kv->list, kv->rows, seqs, table_width, 0, table_width, kv->cfg.n_pages, kv->page_shift, kv->status};
+    compact_kernel<<<1, kPageThreads, size_t(kv->cfg.n_pages + 31) / 32 * 4, st>>>(a);
+    KV_CUDA(cudaGetLastError());
+    return launch_moves(kv, kv->src, kv->dst, kv->count, kv->cfg.n_pages, st);
+}
+
+int ffnrm_kv_copy_pages(ffnrm_kv *kv, const int32_t *src, const int32_t *dst, int n, void *stream) {
+    if (!kv) return fail(FFNRM_ERR_ARG, "null cache");
+    if (n < 0 || n > kv->cfg.n_pages) return fail(FFNRM_ERR_ARG, "n=%d outside [0, n_pages=%d]", n, kv->cfg.n_pages);
+    if (n == 0) return FFNRM_OK;
+    if (!src || !dst || !aligned(src, 4) || !aligned(dst, 4)) return fail(FFNRM_ERR_ARG, "null or misaligned page lists");
+    DeviceGuard guard(kv->device);
+    return launch_moves(kv, src, dst, nullptr, n, static_cast<cudaStream_t>(stream));
+}
+
+int ffnrm_kv_check(ffnrm_kv *kv, void *stream) {
+    if (!kv) return fail(FFNRM_ERR_ARG, "null cache");
+    DeviceGuard guard(kv->device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int bits = 0;
+    KV_CUDA(cudaMemcpyAsync(&bits, kv->status, sizeof(int), cudaMemcpyDeviceToHost, st));
+    KV_CUDA(cudaStreamSynchronize(st));
+    if (!bits) return FFNRM_OK;
+    KV_CUDA(cudaMemsetAsync(kv->status, 0, sizeof(int), st));
+    KV_CUDA(cudaStreamSynchronize(st));
+    if (bits & kStatusWait) return fail(FFNRM_ERR_TIMEOUT, "a kernel gave up waiting on a pipeline barrier");
+    if (bits & (kStatusPage | kStatusLength | kStatusRotary))
+        return fail(FFNRM_ERR_STATE, "a step's data could not be used:%s%s%s",
+                    bits & kStatusPage ? " a page id outside the pool;" : "",
+                    bits & kStatusLength ? " lengths, rows or room that do not fit the tables or the rows;" : "",
+                    bits & kStatusRotary ? " a position past the rotary table;" : "");
+    return fail(FFNRM_ERR_NOMEM, "not enough free pages: nothing was forked");
+}
+
+}  // extern "C"

@@ -1,0 +1,332 @@
+// Page bookkeeping of the 8-bit paged cache, on the device: which pages are held follows from the
+// tables alone, so there is no allocator state to keep in step with them.
+//
+// fork: child i becomes parent parents[i]'s sequence with room for extra[i] more tokens (-1: an
+// empty sequence). Full pages are shared. A partial last page is kept by the lowest child that
+// holds it, unless some child holds it as a full page; every other child gets a copy, so an open
+// page is never shared. New pages are the lowest free ids, in child order.
+// compact: with U pages held, the k-th held page at or above U moves to the k-th free page below
+// U. A moved page never lands on a held one, so the old tables stay readable.
+#pragma once
+
+#include "kv_common.cuh"
+
+namespace ffnrm::kv {
+
+constexpr int kPageThreads = 1024;
+constexpr int kInfoUsed = 0, kInfoFree = 1, kInfoMoved = 2, kInfoShort = 3;
+
+struct PageArgs {
+    const int32_t *tables, *lengths;  // [seqs][width], [seqs]
+    const int32_t *parents, *extra;   // fork: [children]
+    int32_t *out_tables;              // [children or seqs][out_width]
+    int32_t *out_lengths;             // fork: [children]
+    int32_t *info;                    // [4]: pages held, pages free, pages copied or moved, pages short
+    int32_t *src, *dst, *count;       // the moves, for move_kernel
+    int32_t *owner, *list;            // scratch, [pages] each
+    int32_t *rows;                    // scratch, [4][children]
+    int seqs, width, children, out_width, pages, page_shift;
+    int *status;
+};
+
+// Exclusive scan of one value per thread over the block; `total` is the sum.
+__device__ __forceinline__ int block_scan(int v, int &total) {
+    __shared__ int sums[kPageThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        int y = sums[lane];
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) y += z;
+        }
+        sums[lane] = y;
+    }
+    __syncthreads();
+    total = sums[kPageThreads / 32 - 1];
+    return x - v + (warp ? sums[warp - 1] : 0);
+}
+
+// ORs the status bits of all threads (a barrier).
+__device__ __forceinline__ int block_or(int bits, int *shared) {
+    if (bits) atomicOr(shared, bits);
+    __syncthreads();
+    return *shared;
+}
+
+// One block. Shared memory: a bit per page.
+__global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
+    extern __shared__ uint32_t held[];
+    __shared__ int flags;
+    const int words = (a.pages + 31) / 32, P = 1 << a.page_shift, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int32_t *full = a.rows, *open = full + a.children, *need = open + a.children, *from = need + a.children;
+    for (int i = tid; i < words; i += kPageThreads) held[i] = 0;
+    if (tid == 0) flags = 0;
+    __syncthreads();
+    int bad = 0;
+    // each child's parent, full pages and open page
+    for (int c = tid; c < a.children; c += kPageThreads) {
+        const int p = a.parents[c], more = a.extra[c];
+        int length = 0, parent = -1;
+        if (p >= 0 && p < a.seqs) {
+            length = a.lengths[p];
+            if (length >= 0 && length <= (int64_t(a.width) << a.page_shift) && length <= (int64_t(a.out_width) << a.page_shift))
+                parent = p;
+            else {
+                length = 0;
+                bad |= kStatusLength;
+            }
+        } else if (p != -1) {
+            bad |= kStatusLength;
+        }
+        const int nf = length >> a.page_shift;
+        int op = -1;
+        if (parent >= 0 && (length & (P - 1))) {
+            op = a.tables[int64_t(parent) * a.width + nf];
+            if (op < 0 || op >= a.pages) {
+                bad |= kStatusPage;
+                op = -1;
+            }
+        }
+        if (op >= 0) a.owner[op] = 0x7fffffff;
+        int grow = more;
+        if (more < 0 || int64_t(length) + more > (int64_t(a.out_width) << a.page_shift)) {
+            bad |= kStatusLength;
+            grow = 0;
+        }
+        from[c] = parent;
+        full[c] = nf;
+        open[c] = op;
+        need[c] = ((length + grow + P - 1) >> a.page_shift) - nf;
+        a.out_lengths[c] = length + grow;
+    }
+    block_or(bad, &flags);
+    // shared pages
+    for (int c = warp; c < a.children; c += kPageThreads / 32) {
+        const int p = from[c], nf = full[c];
+        if (p < 0) continue;
+        for (int w = lane; w < nf; w += 32) {
+            int id = a.tables[int64_t(p) * a.width + w];
+            if (id >= 0 && id < a.pages)
+                atomicOr(&held[id >> 5], 1u << (id & 31));
+            else {
+                bad |= kStatusPage;
+                id = -1;
+            }
+            a.out_tables[int64_t(c) * a.out_width + w] = id;
+        }
+        if (lane == 0 && open[c] >= 0) atomicMin(&a.owner[open[c]], c);
+    }
+    bad = block_or(bad, &flags);
+    // who keeps an open page; decided before any of them is marked
+    for (int c = tid; c < a.children; c += kPageThreads) {
+        const int op = open[c];
+        if (op < 0) continue;
+        const bool keep = __ldcg(&a.owner[op]) == c && !((held[op >> 5] >> (op & 31)) & 1);
+        if (keep) {
+            need[c] -= 1;
+            full[c] |= int(0x80000000);  // the open page is kept
+        }
+    }
+    __syncthreads();
+    for (int c = tid; c < a.children; c += kPageThreads)
+        if (open[c] >= 0 && full[c] < 0) atomicOr(&held[open[c] >> 5], 1u << (open[c] & 31));
+    __syncthreads();
+    // free pages in ascending order
+    const int per = (words + kPageThreads - 1) / kPageThreads, w0 = tid * per, w1 = min(words, w0 + per);
+    auto free_bits = [&](int w) {
+        const int n = a.pages - w * 32;
+        return ~held[w] & (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+    };
+    int mine = 0, free_total, want = 0, want_total;
+    for (int w = w0; w < w1; ++w) mine += __popc(free_bits(w));
+    int rank = block_scan(mine, free_total);
+    const int cper = (a.children + kPageThreads - 1) / kPageThreads, c0 = tid * cper, c1 = min(a.children, c0 + cper);
+    int copies = 0, copies_total;
+    for (int c = c0; c < c1; ++c) {
+        want += need[c];
+        copies += open[c] >= 0 && full[c] >= 0;
+    }
+    int offset = block_scan(want, want_total);
+    int copy_at = block_scan(copies, copies_total);
+    const int shortage = max(0, want_total - free_total);
+    const bool refuse = shortage || bad;
+    for (int w = w0; w < w1 && rank < want_total; ++w) {
+        for (uint32_t b = free_bits(w); b; b &= b - 1) {
+            if (rank < want_total) a.list[rank] = w * 32 + __ffs(b) - 1;
+            ++rank;
+        }
+    }
+    __syncthreads();
+    for (int c = c0; c < c1; ++c) {
+        const int n = need[c];
+        if (open[c] >= 0 && full[c] >= 0 && !refuse) {
+            a.src[copy_at] = open[c];
+            a.dst[copy_at] = a.list[offset];
+            ++copy_at;
+        }
+        need[c] = offset;
+        offset += n;
+        if (refuse) a.out_lengths[c] = 0;
+    }
+    if (tid == 0) {
+        a.info[kInfoUsed] = a.pages - free_total + (refuse ? 0 : want_total);
+        a.info[kInfoFree] = free_total - (refuse ? 0 : want_total);
+        a.info[kInfoMoved] = refuse ? 0 : copies_total;
+        a.info[kInfoShort] = shortage;
+        *a.count = refuse ? 0 : copies_total;
+        if (refuse) atomicOr(a.status, bad | (shortage ? kStatusPages : 0));
+    }
+    __syncthreads();
+    // the rest of each row: the open page or its copy, new pages, none
+    for (int c = warp; c < a.children; c += kPageThreads / 32) {
+        const bool keep = full[c] < 0;
+        const int nf = full[c] & 0x7fffffff;
+        const int end = (a.out_lengths[c] + P - 1) >> a.page_shift;
+        for (int w = refuse ? lane : nf + lane; w < a.out_width; w += 32) {
+            int id = -1;
+            if (!refuse && w < end) id = keep ? (w == nf ? open[c] : a.list[need[c] + w - nf - 1]) : a.list[need[c] + w - nf];
+            a.out_tables[int64_t(c) * a.out_width + w] = id;
+        }
+    }
+}
+
+// One block. Shared memory: a bit per page.
+__global__ void __launch_bounds__(kPageThreads) compact_kernel(PageArgs a) {
+    extern __shared__ uint32_t held[];
+    __shared__ int flags;
+    const int words = (a.pages + 31) / 32, P = 1 << a.page_shift, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < words; i += kPageThreads) held[i] = 0;
+    if (tid == 0) flags = 0;
+    __syncthreads();
+    int bad = 0;
+    for (int s = warp; s < a.seqs; s += kPageThreads / 32) {
+        int length = a.lengths[s];
+        if (length < 0 || length > (int64_t(a.width) << a.page_shift)) {
+            bad |= kStatusLength;
+            length = 0;
+        }
+        const int n = (length + P - 1) >> a.page_shift;
+        for (int w = lane; w < n; w += 32) {
+            const int id = a.tables[int64_t(s) * a.width + w];
+            if (id >= 0 && id < a.pages)
+                atomicOr(&held[id >> 5], 1u << (id & 31));
+            else
+                bad |= kStatusPage;
+        }
+    }
+    bad = block_or(bad, &flags);
+    const int per = (words + kPageThreads - 1) / kPageThreads, w0 = tid * per, w1 = min(words, w0 + per);
+    int mine = 0, used;
+    for (int w = w0; w < w1; ++w) mine += __popc(held[w]);
+    int before = block_scan(mine, used);  // held pages below this thread's words
+    // holes below `used` in order, then the held pages at or above it
+    for (int w = w0; w < w1; ++w) {
+        const int inside = used - w * 32;
+        if (inside <= 0) break;
+        uint32_t b = ~held[w] & (inside >= 32 ? 0xffffffffu : (1u << inside) - 1u);
+        int rank = w * 32 - before;
+        before += __popc(held[w]);
+        for (; b; b &= b - 1) a.list[rank++] = w * 32 + __ffs(b) - 1;
+    }
+    __syncthreads();
+    // held pages below `used`, so that those above can be ranked
+    int low = 0, low_total, high = 0, high_total;
+    for (int w = w0; w < w1; ++w) {
+        const int inside = used - w * 32;
+        const uint32_t lowmask = inside <= 0 ? 0u : inside >= 32 ? 0xffffffffu : (1u << inside) - 1u;
+        low += __popc(held[w] & lowmask);
+        high += __popc(held[w] & ~lowmask);
+    }
+    block_scan(low, low_total);
+    int rank = block_scan(high, high_total);
+    for (int w = w0; w < w1; ++w) {
+        const int inside = used - w * 32;
+        const uint32_t lowmask = inside <= 0 ? 0u : inside >= 32 ? 0xffffffffu : (1u << inside) - 1u;
+        for (uint32_t b = held[w] & ~lowmask; b; b &= b - 1) {
+            const int id = w * 32 + __ffs(b) - 1, to = a.list[rank];
+            a.owner[id] = to;
+            if (!bad) {
+                a.src[rank] = id;
+                a.dst[rank] = to;
+            }
+            ++rank;
+        }
+    }
+    if (tid == 0) {
+        a.info[kInfoUsed] = used;
+        a.info[kInfoFree] = a.pages - used;
+        a.info[kInfoMoved] = bad ? 0 : high_total;
+        a.info[kInfoShort] = 0;
+        *a.count = bad ? 0 : high_total;
+        if (bad) atomicOr(a.status, bad);
+    }
+    __syncthreads();
+    // bad tables: nothing moves and the rows are handed on as they are
+    for (int s = warp; s < a.seqs; s += kPageThreads / 32) {
+        const int length = a.lengths[s];
+        const int n = bad ? a.width : (length + P - 1) >> a.page_shift;
+        for (int w = lane; w < a.width; w += 32) {
+            int id = -1;
+            if (w < n) {
+                id = a.tables[int64_t(s) * a.width + w];
+                if (!bad && id >= used) id = __ldcg(&a.owner[id]);
+            }
+            a.out_tables[int64_t(s) * a.width + w] = id;
+        }
+    }
+}
+
+struct MoveArgs {
+    int8_t *k_codes, *v_codes;   // all layers
+    float *k_scale, *v_scale;
+    const int32_t *src, *dst, *count;
+    int layers, pages, heads, page_bytes;  // page_bytes: codes of one page of one layer
+    int most;                              // upper bound of the list; its length without a count
+    int *status;
+};
+
+constexpr int kMoveChunk = 16384;
+
+// Copies every listed page in every layer, kMoveChunk bytes of codes per block step.
+__global__ void __launch_bounds__(256) move_kernel(MoveArgs a) {
+    const int moves = a.count ? min(*a.count, a.most) : a.most, chunks = (a.page_bytes + kMoveChunk - 1) / kMoveChunk;
+    const int64_t items = int64_t(moves) * a.layers * 2 * chunks;
+    for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        const int chunk = int(i % chunks);
+        int64_t r = i / chunks;
+        const int kv = int(r & 1);
+        r >>= 1;
+        const int layer = int(r % a.layers), m = int(r / a.layers);
+        const int src = a.src[m], dst = a.dst[m];
+        if (src < 0 || src >= a.pages || dst < 0 || dst >= a.pages) {
+            if (threadIdx.x == 0) atomicOr(a.status, kStatusPage);
+            continue;
+        }
+        const int64_t from = int64_t(layer) * a.pages + src, to = int64_t(layer) * a.pages + dst;
+        int8_t *codes = kv ? a.v_codes : a.k_codes;
+        const uint4 *x = reinterpret_cast<const uint4 *>(codes + from * a.page_bytes + int64_t(chunk) * kMoveChunk);
+        uint4 *y = reinterpret_cast<uint4 *>(codes + to * a.page_bytes + int64_t(chunk) * kMoveChunk);
+        const int n = min(kMoveChunk, a.page_bytes - chunk * kMoveChunk) / 16;
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (int(threadIdx.x) + j * 256 < n) v[j] = x[threadIdx.x + j * 256];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (int(threadIdx.x) + j * 256 < n) y[threadIdx.x + j * 256] = v[j];
+        if (chunk == 0) {
+            float *scale = kv ? a.v_scale : a.k_scale;
+            for (int h = threadIdx.x; h < a.heads; h += 256) scale[to * a.heads + h] = scale[from * a.heads + h];
+        }
+    }
+}
+
+}  // namespace ffnrm::kv

@@ -1,0 +1,357 @@
+"""The attention half of a decoder layer next to the split FFN: rotary positions and an
+8-bit paged cache (append, attend, read, fork, compact) over the C ABI.
+
+A cache holds K and V as int8 codes in pages of ``page_tokens`` tokens, with one f32 scale
+for each page and head (value = code * scale). A step works on a batch of sequences given by
+three int32 device tensors:
+
+* ``tables``  [seqs, width]  page ids of each sequence in order;
+* ``lengths`` [seqs]         tokens it holds, the step's new ones included (0: an idle slot);
+* ``starts``  [seqs + 1]     rows of its new tokens in q, k and v (None: one row each).
+
+The j-th of a sequence's n new tokens stands at position ``lengths - n + j``. A step is then:
+``fork`` (reserve room; also shares, copies and frees pages between steps), and per layer
+``append`` (rotates q and k, quantises k and v into the pages) and ``attend``.
+
+Arguments are torch tensors on the cache's device. Shape and type errors raise
+``ValueError``; data on the device that a kernel could not use is recorded and raised by
+``check``. Calls run on the current stream (or ``stream``) without synchronising and can be
+captured in a CUDA graph; calls on one cache must not overlap on the GPU.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+from . import _native as N
+from .engine import _stream
+
+
+def _dtype(x) -> int:
+    import torch
+    try:
+        return {torch.float16: N.F16, torch.bfloat16: N.BF16, torch.float32: N.F32}[x.dtype]
+    except KeyError:
+        raise ValueError(f"expected float16, bfloat16 or float32, got {x.dtype}") from None
+
+
+def _on(name, x, device):
+    if x.device != device:
+        raise ValueError(f"{name} must be on {device}, got {x.device}")
+
+
+def _rows(name, x, heads, dim, rows=None) -> N.Rows:
+    """A [rows, heads, dim] view with contiguous channels."""
+    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != dim or (rows is not None and x.shape[0] != rows):
+        raise ValueError(f"{name} must have shape ({'T' if rows is None else rows}, {heads}, {dim}), got {tuple(x.shape)}")
+    if x.stride(2) != 1 and dim > 1 and x.numel():
+        raise ValueError(f"{name} must have contiguous channels")
+    return N.Rows(x.data_ptr(), x.stride(0), x.stride(1))
+
+
+def _writable(name, x):
+    """A tensor that is written must not name one element twice (an expanded view)."""
+    if any(st == 0 and n > 1 for st, n in zip(x.stride(), x.shape)):
+        raise ValueError(f"{name} must not be an expanded view")
+
+
+def _ints(name, x, shape, device):
+    import torch
+    if x.dtype != torch.int32 or tuple(x.shape) != tuple(shape) or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}, got {x.dtype} {tuple(x.shape)}")
+    _on(name, x, device)
+    return x.data_ptr()
+
+
+class RotaryTable:
+    """Cosines and sines of every position, f32 [max_positions, rotary_dim] (cosines, then
+    sines). Pair i of a head turns by ``position * base ** (-2 i / rotary_dim)``.
+
+    ``scaling`` for contexts longer than the weights were trained on:
+
+    * ``"linear"`` — positions divided by ``factor``;
+    * ``"ntk"`` — the base raised to ``base * factor ** (R / (R - 2))``, which leaves the
+      fastest pair as it is and slows the slowest one by ``factor``;
+    * ``"yarn"`` — per pair: pairs that turn more than ``beta_fast`` times within
+      ``original_positions`` stay, those below ``beta_slow`` turns are divided by
+      ``factor``, a ramp between; cosines and sines are multiplied by
+      ``0.1 ln(factor) + 1`` (YaRN, Peng et al. 2023).
+    """
+
+    def __init__(self, rotary_dim: int, max_positions: int, base: float = 10000.0, interleaved: bool = False,
+                 scaling: str | None = None, factor: float = 1.0, original_positions: int | None = None,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, device=0):
+        import torch
+        if rotary_dim <= 0 or rotary_dim % 2 or max_positions <= 0:
+            raise ValueError("rotary_dim must be even and positive, max_positions positive")
+        if scaling not in (None, "linear", "ntk", "yarn"):
+            raise ValueError(f"unknown scaling {scaling!r}")
+        if scaling is not None and factor < 1.0:
+            raise ValueError("factor must be at least 1")
+        if base <= 1.0:
+            raise ValueError("base must be above 1")
+        pair = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+        gain = 1.0
+        if scaling == "ntk" and rotary_dim > 2:
+            base = base * factor ** (rotary_dim / (rotary_dim - 2))
+        freq = base ** (-pair / rotary_dim)
+        if scaling == "linear":
+            freq = freq / factor
+        elif scaling == "yarn":
+            if not original_positions or original_positions <= 0 or beta_fast <= beta_slow:
+                raise ValueError("yarn needs original_positions and beta_fast > beta_slow")
+            # the (fractional) pair that makes `turns` turns within the original context
+            at = [rotary_dim * math.log(original_positions / (turns * 2 * math.pi)) / (2 * math.log(base))
+                  for turns in (beta_fast, beta_slow)]
+            low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary_dim // 2 - 1)
+            ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+            freq = freq * (1 - ramp) + freq / factor * ramp
+            gain = 0.1 * math.log(factor) + 1.0
+        angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * freq
+        self._set((torch.cat([angle.cos(), angle.sin()], 1) * gain).float().to(
+            torch.device("cuda", device) if isinstance(device, int) else device), interleaved)
+
+    @classmethod
+    def from_tensor(cls, cos_sin, interleaved: bool = False) -> "RotaryTable":
+        """A table of the caller's own angles: f32 [max_positions, rotary_dim]."""
+        self = cls.__new__(cls)
+        self._set(cos_sin, interleaved)
+        return self
+
+    def _set(self, cos_sin, interleaved):
+        import torch
+        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.shape[1] % 2 \
+                or 0 in cos_sin.shape:
+            raise ValueError("cos_sin must be a contiguous float32 tensor [max_positions, rotary_dim]")
+        self.cos_sin, self.interleaved = cos_sin, bool(interleaved)
+        self.max_positions, self.rotary_dim = cos_sin.shape
+        self.flags = N.ROTARY_INTERLEAVED if interleaved else 0
+
+
+def rotary(x, positions, table: RotaryTable, out=None, inverse: bool = False, stream=None):
+    """x [T, heads, dim] with its first ``rotary_dim`` channels rotated at ``positions`` (int32
+    [T]); ``inverse`` applies the transposed rotation, the gradient of the forward one.
+    ``out`` may be x. A position outside the table gives NaN in the rotated channels."""
+    import torch
+    if x.dim() != 3:
+        raise ValueError(f"x must have shape (T, heads, dim), got {tuple(x.shape)}")
+    T, heads, dim = x.shape
+    if table.rotary_dim > dim:
+        raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head dim {dim}")
+    if out is None:
+        out = torch.empty((T, heads, dim), dtype=x.dtype, device=x.device)
+    if out.dtype != x.dtype or out.shape != x.shape:
+        raise ValueError("out must have x's type and shape")
+    _writable("out", out)
+    for name, t in (("out", out), ("table", table.cos_sin)):
+        _on(name, t, x.device)
+    dtype, xr, yr = _dtype(x), _rows("x", x, heads, dim), _rows("out", out, heads, dim)
+    pos = _ints("positions", positions, (T,), x.device)
+    with torch.cuda.device(x.device):
+        N.check(N.lib().ffnrm_rotary(ctypes.byref(xr), ctypes.byref(yr), dtype, T, heads, dim, pos,
+                                     table.cos_sin.data_ptr(), table.rotary_dim, table.max_positions,
+                                     table.flags | (N.ROTARY_INVERSE if inverse else 0), _stream(stream)))
+    return out
+
+
+class PagedKvCache:
+    """K and V of ``n_layers`` layers in ``n_pages`` pages of ``page_tokens`` tokens each.
+
+    ``buffers``: (k_codes, v_codes, k_scale, v_scale) to use in place of new ones: int8
+    [layers, pages, kv_heads, page_tokens, head_dim] and f32 [layers, pages, kv_heads].
+    """
+
+    def __init__(self, n_layers: int, n_pages: int, kv_heads: int, head_dim: int, page_tokens: int = 64,
+                 max_seqs: int = 256, device: int = 0, buffers=None):
+        import torch
+        self.handle = None
+        self.lib = N.lib()
+        self.n_layers, self.n_pages, self.kv_heads, self.head_dim = n_layers, n_pages, kv_heads, head_dim
+        self.page_tokens, self.max_seqs = page_tokens, max_seqs
+        self.device = torch.device("cuda", device)
+        if min(n_layers, n_pages, kv_heads, max_seqs) <= 0 or head_dim not in (64, 128, 256) \
+                or page_tokens not in (16, 32, 64, 128):
+            raise ValueError(f"n_layers={n_layers}, n_pages={n_pages}, kv_heads={kv_heads}, max_seqs={max_seqs} must be "
+                             f"positive, head_dim={head_dim} 64, 128 or 256, page_tokens={page_tokens} 16, 32, 64 or 128")
+        codes, scale = (n_layers, n_pages, kv_heads, page_tokens, head_dim), (n_layers, n_pages, kv_heads)
+        if buffers is None:
+            buffers = [torch.zeros(codes, dtype=torch.int8, device=self.device) for _ in range(2)] + \
+                      [torch.zeros(scale, dtype=torch.float32, device=self.device) for _ in range(2)]
+            torch.cuda.current_stream(self.device).synchronize()
+        for b, shape, dtype in zip(buffers, (codes, codes, scale, scale), (torch.int8, torch.int8, torch.float32, torch.float32)):
+            if tuple(b.shape) != shape or b.dtype != dtype or not b.is_contiguous():
+                raise ValueError(f"a cache buffer must be a contiguous {dtype} tensor of shape {shape}, "
+                                 f"got {b.dtype} {tuple(b.shape)}")
+            _on("a cache buffer", b, self.device)
+        self.k_codes, self.v_codes, self.k_scale, self.v_scale = buffers
+        cfg = N.KvConfig(n_layers, n_pages, kv_heads, head_dim, page_tokens, max_seqs)
+        handle = ctypes.c_void_p()
+        N.check(self.lib.ffnrm_kv_create(ctypes.byref(handle), device, ctypes.byref(cfg),
+                                         *(b.data_ptr() for b in buffers)))
+        self.handle = handle
+
+    # -- lifetime ---------------------------------------------------------
+    def close(self) -> None:
+        if getattr(self, "handle", None):
+            N.check(self.lib.ffnrm_kv_destroy(self.handle))
+            self.handle = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def check(self, stream=None) -> None:
+        """Synchronise and raise what the kernels recorded: MemoryError (too few free pages),
+        TimeoutError (a bounded wait ran out), RuntimeError (data that could not be used)."""
+        N.check(self.lib.ffnrm_kv_check(self.handle, self._stream(stream)))
+
+    def _stream(self, stream):
+        import torch
+        return _stream(torch.cuda.current_stream(self.device) if stream is None else stream)
+
+    def _batch(self, tables, lengths, starts, rows) -> N.KvBatch:
+        if tables.dim() != 2:
+            raise ValueError(f"tables must have shape (seqs, width), got {tuple(tables.shape)}")
+        seqs, width = tables.shape
+        return N.KvBatch(_ints("tables", tables, (seqs, width), self.device),
+                         _ints("lengths", lengths, (seqs,), self.device),
+                         None if starts is None else _ints("starts", starts, (seqs + 1,), self.device), seqs, width, rows)
+
+    # -- a step's work --------------------------------------------------------
+    def append(self, layer: int, k, v, tables, lengths, starts=None, rope: RotaryTable | None = None, q=None, q_out=None,
+               stream=None):
+        """Quantise the step's new k and v [T, kv_heads, head_dim] into their pages. With
+        ``rope`` the keys are rotated at their positions first, and with ``q`` [T, heads,
+        head_dim] the queries too; returns the rotated queries (``q_out``, which may be q)."""
+        import torch
+        T = k.shape[0] if k.dim() == 3 else -1
+        kr, vr = _rows("k", k, self.kv_heads, self.head_dim), _rows("v", v, self.kv_heads, self.head_dim, T)
+        dtype = _dtype(k)
+        if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+            raise ValueError("q, k and v must have one type")
+        batch = self._batch(tables, lengths, starts, T)
+        for name, t in (("k", k), ("v", v)):
+            _on(name, t, self.device)
+        qr = yr = None
+        q_heads = 0
+        if q is not None:
+            if rope is None:
+                raise ValueError("q is only rotated: it needs rope")
+            q_heads = q.shape[1] if q.dim() == 3 else -1
+            qr = _rows("q", q, q_heads, self.head_dim, T)
+            _on("q", q, self.device)
+            if q_out is None:
+                q_out = torch.empty((T, q_heads, self.head_dim), dtype=q.dtype, device=self.device)
+            yr = _rows("q_out", q_out, q_heads, self.head_dim, T)
+            _on("q_out", q_out, self.device)
+            _writable("q_out", q_out)
+            if q_out.dtype != q.dtype:
+                raise ValueError("q_out must have q's type")
+        if rope is not None:
+            _on("rope", rope.cos_sin, self.device)
+        N.check(self.lib.ffnrm_kv_append(
+            self.handle, layer, ctypes.byref(batch), dtype, ctypes.byref(kr), ctypes.byref(vr),
+            ctypes.byref(qr) if qr else None, ctypes.byref(yr) if yr else None, q_heads,
+            rope.cos_sin.data_ptr() if rope else None, rope.rotary_dim if rope else 0, rope.max_positions if rope else 0,
+            rope.flags if rope else 0, self._stream(stream)))
+        return q_out
+
+    def attend(self, layer: int, q, tables, lengths, starts=None, out=None, lse=None, scale: float | None = None,
+               causal: bool = True, window: int = 0, stream=None):
+        """Attention of the step's queries q [T, heads, head_dim] (float16 or bfloat16) over the
+        cache, the step's own tokens included. ``scale`` defaults to ``head_dim ** -0.5``;
+        ``window`` > 0 lets a query see its last ``window`` positions only. ``lse`` (float32
+        [T, heads]) receives the natural log of the sum of exponentials."""
+        import torch
+        if q.dim() != 3 or q.shape[1] % self.kv_heads or q.shape[1] == 0:
+            raise ValueError(f"q must have shape (T, a multiple of {self.kv_heads}, {self.head_dim}), got {tuple(q.shape)}")
+        T, heads = q.shape[:2]
+        dtype, qr = _dtype(q), _rows("q", q, heads, self.head_dim)
+        batch = self._batch(tables, lengths, starts, T)
+        if out is None:
+            out = torch.empty((T, heads, self.head_dim), dtype=q.dtype, device=self.device)
+        yr = _rows("out", out, heads, self.head_dim, T)
+        for name, t in (("q", q), ("out", out)):
+            _on(name, t, self.device)
+        _writable("out", out)
+        if out.dtype != q.dtype:
+            raise ValueError("out must have q's type")
+        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (T, heads) or not lse.is_contiguous()):
+            raise ValueError(f"lse must be a contiguous float32 tensor of shape ({T}, {heads})")
+        if lse is not None:
+            _on("lse", lse, self.device)
+        N.check(self.lib.ffnrm_kv_attend(
+            self.handle, layer, ctypes.byref(batch), dtype, ctypes.byref(qr), ctypes.byref(yr),
+            None if lse is None else lse.data_ptr(), heads, self.head_dim ** -0.5 if scale is None else float(scale),
+            int(bool(causal)), int(window), self._stream(stream)))
+        return out
+
+    def read(self, layer: int, tables, lengths, starts, rows: int, dtype=None, stream=None):
+        """The last tokens of each sequence back from the cache: k and v [rows, kv_heads,
+        head_dim] (code * scale), float32 unless ``dtype``. ``starts`` says how many of each."""
+        import torch
+        dtype = torch.float32 if dtype is None else dtype
+        batch = self._batch(tables, lengths, starts, rows)
+        k, v = (torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
+        N.check(self.lib.ffnrm_kv_read(self.handle, layer, ctypes.byref(batch), _dtype(k), k.data_ptr(), v.data_ptr(),
+                                       self._stream(stream)))
+        return k, v
+
+    # -- pages between steps --------------------------------------------------
+    def fork(self, tables, lengths, parents, extra, out_tables=None, out_lengths=None, info=None, stream=None):
+        """The next step's batch: child i continues sequence ``parents[i]`` (-1: an empty one)
+        with room for ``extra[i]`` new tokens. A sequence named by several children is
+        shared (its open last page is copied), one named by none is freed. Returns (tables,
+        lengths, info); info int32 [4] holds the pages held, free, copied and short."""
+        import torch
+        if tables.dim() != 2 or parents.dim() != 1:
+            raise ValueError("tables must have shape (seqs, width), parents (children,)")
+        seqs, width = tables.shape
+        n = parents.shape[0]
+        if out_tables is None:
+            out_tables = torch.empty((n, width), dtype=torch.int32, device=self.device)
+        if out_lengths is None:
+            out_lengths = torch.empty((n,), dtype=torch.int32, device=self.device)
+        if info is None:
+            info = torch.empty((4,), dtype=torch.int32, device=self.device)
+        if out_tables.dim() != 2:
+            raise ValueError("out_tables must have shape (children, width)")
+        d = self.device
+        N.check(self.lib.ffnrm_kv_fork(
+            self.handle, _ints("tables", tables, (seqs, width), d), _ints("lengths", lengths, (seqs,), d), seqs, width,
+            _ints("parents", parents, (n,), d), _ints("extra", extra, (n,), d), n,
+            _ints("out_tables", out_tables, (n, out_tables.shape[1]), d), out_tables.shape[1],
+            _ints("out_lengths", out_lengths, (n,), d), _ints("info", info, (4,), d), self._stream(stream)))
+        return out_tables, out_lengths, info
+
+    def compact(self, tables, lengths, out_tables=None, info=None, stream=None):
+        """Move the held pages to the lowest ids. Returns (tables, info); ``out_tables`` may be
+        ``tables``. No held page is overwritten, so the old tables stay readable until the
+        next fork hands out the freed pages."""
+        import torch
+        if tables.dim() != 2:
+            raise ValueError("tables must have shape (seqs, width)")
+        seqs, width = tables.shape
+        if out_tables is None:
+            out_tables = torch.empty_like(tables)
+        if info is None:
+            info = torch.empty((4,), dtype=torch.int32, device=self.device)
+        d = self.device
+        N.check(self.lib.ffnrm_kv_compact(
+            self.handle, _ints("tables", tables, (seqs, width), d), _ints("lengths", lengths, (seqs,), d), seqs, width,
+            _ints("out_tables", out_tables, (seqs, width), d), _ints("info", info, (4,), d), self._stream(stream)))
+        return out_tables, info
+
+    def copy_pages(self, src, dst, stream=None) -> None:
+        """Copy page src[i] to dst[i] in every layer (int32 [n]; no page is named twice)."""
+        n = src.shape[0] if src.dim() == 1 else -1
+        N.check(self.lib.ffnrm_kv_copy_pages(self.handle, _ints("src", src, (n,), self.device),
+                                             _ints("dst", dst, (n,), self.device), n, self._stream(stream)))

@@ -273,6 +273,109 @@ int ffnrm_base_from_table(ffnrm_base_producer *p, const ffnrm_radix_table *table
 /* The exact integer dots P_hi [rows, hidden/32] of one token (verification). */
 int ffnrm_table_dots(const ffnrm_radix_table *table, const int8_t *z, int32_t *dots);
 
+/* ---- Attention half of a decoder layer on an 8-bit paged cache ----------------------
+ * No counterpart in the reference, which serves the FFN half; these entry points run the
+ * rest of a decoder layer's per-token work next to it. All pointers are device memory on
+ * the current (ffnrm_rotary) or the handle's device; element types are FFNRM_F16 /
+ * FFNRM_BF16 / FFNRM_F32, and a row block [rows][heads][dim] is given by its base and its
+ * token and head strides in elements (channels are contiguous). */
+#define FFNRM_F16 0
+#define FFNRM_BF16 1
+#define FFNRM_F32 2
+typedef struct {
+    void *data;
+    int64_t token_stride, head_stride;
+} ffnrm_rows;
+
+/* Rotary positions: y = x with its first rotary_dim channels rotated by row positions[t]
+ * of `table` f32 [max_positions][rotary_dim] (rotary_dim/2 cosines, then the sines). Pair i
+ * is channels (i, i + rotary_dim/2), or (2i, 2i + 1) with FFNRM_ROTARY_INTERLEAVED;
+ * FFNRM_ROTARY_INVERSE applies the transposed rotation (the gradient). f32 arithmetic, one
+ * rounding. y may be x. A position outside the table gives NaN in the rotated channels. */
+#define FFNRM_ROTARY_INTERLEAVED 1
+#define FFNRM_ROTARY_INVERSE 2
+int ffnrm_rotary(const ffnrm_rows *x, const ffnrm_rows *y, int dtype, int tokens, int heads, int head_dim,
+                 const int32_t *positions, const float *table, int rotary_dim, int max_positions, int flags,
+                 void *stream);
+
+/* A cache of K and V as int8 codes in pages, with one f32 scale for each page and head:
+ *   codes [n_layers][n_pages][kv_heads][page_tokens][head_dim], scales [n_layers][n_pages][kv_heads],
+ *   value = code * scale.
+ * The four pools are the caller's device memory (codes 16-byte aligned), borrowed for the
+ * handle's life. The handle owns a workspace: its calls must not overlap on the GPU (one
+ * stream, or ordered by events), like a context's. All calls are asynchronous and
+ * capturable. Data on the device that cannot be used (a page id outside the pool, a length
+ * that does not fit) is skipped and recorded; ffnrm_kv_check reports it. */
+typedef struct ffnrm_kv ffnrm_kv;
+typedef struct {
+    int32_t n_layers;
+    int32_t n_pages;     /* up to 1048576 */
+    int32_t kv_heads;
+    int32_t head_dim;    /* 64, 128 or 256 */
+    int32_t page_tokens; /* 16, 32, 64 or 128 */
+    int32_t max_seqs;    /* largest batch of any call, up to 4096 */
+} ffnrm_kv_config;
+/* One step's batch, all device memory. tables [seqs][table_width] page ids; lengths [seqs]
+ * tokens held, the step's new ones included; starts [seqs + 1] the rows of the new tokens
+ * (NULL: one row per sequence, rows = seqs). The j-th of a sequence's n rows stands at
+ * position lengths - n + j. A sequence of length 0 is an idle slot. */
+typedef struct {
+    const int32_t *tables, *lengths, *starts;
+    int32_t seqs, table_width, rows;
+} ffnrm_kv_batch;
+int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8_t *k_codes, int8_t *v_codes,
+                    float *k_scale, float *v_scale);
+int ffnrm_kv_destroy(ffnrm_kv *kv);
+
+/* Write a step's new keys and values k, v [rows][kv_heads][head_dim] (any of the three
+ * types) into the pages. Per touched page and head: s = max(s_old, max|x_new| / 127, 1e-12)
+ * with s_old the scale where the page already holds earlier tokens; earlier codes become
+ * rint(q * (s_old / s)), new ones rint(x / s). Non-finite values make the scale NaN. With
+ * `table` the keys are rotated at their positions first, and with q, q_out as well the
+ * queries [rows][q_heads][head_dim] (q_out may be q; rows of idle slots become zeros). */
+int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, const ffnrm_rows *k,
+                    const ffnrm_rows *v, const ffnrm_rows *q, const ffnrm_rows *q_out, int q_heads, const float *table,
+                    int rotary_dim, int max_positions, int flags, void *stream);
+
+/* The batch's rows back from the cache: k, v [rows][kv_heads][head_dim] contiguous,
+ * code * scale in `dtype`. Idle slots read as zeros. */
+int ffnrm_kv_read(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, void *k, void *v, void *stream);
+
+/* Attention of a step's queries q [rows][q_heads][head_dim] (f16 or bf16; q_heads a multiple
+ * of kv_heads) over the cache, its new tokens included: softmax(scale * q k) v over the keys
+ * j <= position (causal, else all) and j > position - window (window > 0). f32 softmax
+ * statistics. lse (optional, f32 [rows][q_heads]): natural log of the sum of exponentials. A
+ * row that sees no key gives zeros and -inf; so do rows of idle slots and past starts[seqs].
+ * A row that sees a token of a page whose scale is NaN is NaN (lse too). Pages that no row
+ * sees (before every window) are not looked up: their table entries may be -1. */
+int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, const ffnrm_rows *q,
+                    const ffnrm_rows *out, float *lse, int q_heads, float scale, int causal, int window, void *stream);
+
+/* Pages between steps. Which pages are held follows from the tables and lengths alone.
+ * fork: child i of `children` becomes the sequence parents[i] with room for extra[i] more
+ * tokens (parents[i] = -1: an empty one; a sequence that no child names is freed). Full
+ * pages are shared; an open last page is kept by one child and copied for the others, in
+ * every layer; new pages are the lowest free ids in child order. out_tables
+ * [children][out_width] (-1 past the end; not the input's memory), out_lengths [children];
+ * info int32 [4]: pages held, free, copied, and short. With too few free pages nothing is
+ * copied, the outputs are empty sequences, info[3] says how many are missing and
+ * ffnrm_kv_check reports FFNRM_ERR_NOMEM; the input tables stay valid.
+ * compact: moves the held pages to the lowest ids, in every layer; out_tables (may be the
+ * input) names the new places; info: pages held, free, moved, 0.
+ * copy_pages: page src[i] to dst[i] for i < n, in every layer (device lists; a page named
+ * as a destination is named once and is no source). */
+int ffnrm_kv_fork(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, int seqs, int table_width,
+                  const int32_t *parents, const int32_t *extra, int children, int32_t *out_tables, int out_width,
+                  int32_t *out_lengths, int32_t *info, void *stream);
+int ffnrm_kv_compact(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, int seqs, int table_width,
+                     int32_t *out_tables, int32_t *info, void *stream);
+int ffnrm_kv_copy_pages(ffnrm_kv *kv, const int32_t *src, const int32_t *dst, int n, void *stream);
+
+/* Synchronises `stream` and reports (and clears) what the handle's kernels recorded since
+ * the last check: FFNRM_ERR_NOMEM too few free pages, FFNRM_ERR_TIMEOUT a bounded wait ran
+ * out, FFNRM_ERR_STATE data that could not be used (the message names it). */
+int ffnrm_kv_check(ffnrm_kv *kv, void *stream);
+
 const char *ffnrm_last_error(void);
 const char *ffnrm_version(void);
 

@@ -1,0 +1,103 @@
+"""Rotary tables and the argument checks of the paged cache that need no GPU."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+
+def angles(table):
+    R = table.rotary_dim
+    c, s = table.cos_sin[:, :R // 2].double(), table.cos_sin[:, R // 2:].double()
+    return np.hypot(c.numpy(), s.numpy()), np.arctan2(s.numpy(), c.numpy())
+
+
+def table(*args, **kw):
+    import torch
+    from ffn_residual_mesh_b200.kvcache import RotaryTable
+    return RotaryTable(*args, device=torch.device("cpu"), **kw)
+
+
+@pytest.mark.parametrize("kind,factor", [(None, 1.0), ("linear", 4.0), ("ntk", 4.0), ("yarn", 8.0)])
+def test_rotary_table(kind, factor):
+    R, n, base, orig = 64, 300, 10000.0, 4096
+    t = table(R, n, base=base, scaling=kind, factor=factor, original_positions=orig)
+    gain, angle = angles(t)
+    want_gain = 0.1 * math.log(factor) + 1 if kind == "yarn" else 1.0
+    assert np.abs(gain - want_gain).max() < 3e-7
+    for i in range(R // 2):
+        f = base ** (-2 * i / R)
+        if kind == "linear":
+            f /= factor
+        elif kind == "ntk":
+            f = (base * factor ** (R / (R - 2))) ** (-2 * i / R)
+        elif kind == "yarn":
+            turns = lambda r: R * math.log(orig / (r * 2 * math.pi)) / (2 * math.log(base))
+            low, high = math.floor(turns(32)), math.ceil(turns(1))
+            ramp = min(max((i - low) / (high - low), 0), 1)
+            f = f * (1 - ramp) + f / factor * ramp
+        p = np.arange(n) * f
+        off = (angle[:, i] - p + math.pi) % (2 * math.pi) - math.pi
+        assert np.abs(off).max() < 1e-6
+    if kind == "ntk":  # the fastest pair as it was, the slowest slowed by the factor
+        assert abs(base ** (-(R - 2) / R) / factor - (base * factor ** (R / (R - 2))) ** (-(R - 2) / R)) < 1e-12
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_dim=3, max_positions=4), dict(rotary_dim=0, max_positions=4), dict(rotary_dim=4, max_positions=0),
+                                dict(rotary_dim=4, max_positions=4, scaling="cubic"), dict(rotary_dim=4, max_positions=4, base=1.0),
+                                dict(rotary_dim=4, max_positions=4, scaling="linear", factor=0.5),
+                                dict(rotary_dim=4, max_positions=4, scaling="yarn", factor=2.0)])
+def test_rotary_table_refuses(kw):
+    with pytest.raises(ValueError):
+        table(**kw)
+
+
+def test_rotary_table_from_tensor_refuses():
+    import torch
+    from ffn_residual_mesh_b200.kvcache import RotaryTable
+    for bad in (torch.zeros(4, 6, dtype=torch.float64), torch.zeros(4, 5), torch.zeros(8), torch.zeros(8, 4)[:, :2], torch.zeros(0, 4)):
+        with pytest.raises(ValueError):
+            RotaryTable.from_tensor(bad)
+
+
+@pytest.mark.parametrize("cfg", [(0, 4, 1, 64, 16, 1), (1, 0, 1, 64, 16, 1), (1, (1 << 20) + 1, 1, 64, 16, 1), (1, 4, 0, 64, 16, 1),
+                                 (1, 4, 1, 96, 16, 1), (1, 4, 1, 64, 24, 1), (1, 4, 1, 64, 256, 1), (1, 4, 1, 64, 16, 0),
+                                 (1, 4, 1, 64, 16, 4097), (1, 4, 2000, 64, 16, 1)])
+def test_create_refuses_shapes_before_any_device(cfg):
+    from ffn_residual_mesh_b200 import _native as N
+    from ffn_residual_mesh_b200 import build
+    build.build()
+    handle = ctypes.c_void_p()
+    rc = N.lib().ffnrm_kv_create(ctypes.byref(handle), 0, ctypes.byref(N.KvConfig(*cfg)), 16, 16, 16, 16)
+    assert rc == N.ERR_ARG and not handle.value
+    with pytest.raises(ValueError):
+        N.check(rc)
+
+
+def test_create_refuses_pools():
+    from ffn_residual_mesh_b200 import _native as N
+    cfg, handle = N.KvConfig(1, 4, 1, 64, 16, 1), ctypes.c_void_p()
+    for pools in ((None, 16, 16, 16), (16, 16, 16, None), (8, 16, 16, 16), (16, 24, 16, 16), (16, 16, 18, 16)):
+        assert N.lib().ffnrm_kv_create(ctypes.byref(handle), 0, ctypes.byref(cfg), *pools) == N.ERR_ARG
+    assert N.lib().ffnrm_kv_create(None, 0, ctypes.byref(cfg), 16, 16, 16, 16) == N.ERR_ARG
+
+
+def test_null_cache_and_rotary_arguments_are_refused():
+    from ffn_residual_mesh_b200 import _native as N
+    lib, null = N.lib(), None
+    batch = N.KvBatch(16, 16, None, 1, 1, 1)
+    rows = N.Rows(64, 64, 64)
+    assert lib.ffnrm_kv_attend(null, 0, ctypes.byref(batch), 0, ctypes.byref(rows), ctypes.byref(rows), None, 1, 1.0, 1, 0, None) == N.ERR_ARG
+    assert lib.ffnrm_kv_check(null, None) == N.ERR_ARG and lib.ffnrm_kv_destroy(null) == N.OK
+    assert lib.ffnrm_kv_copy_pages(null, 16, 16, 1, None) == N.ERR_ARG
+
+    def rotary(x=rows, y=rows, dtype=0, tokens=2, heads=1, dim=64, pos=16, table=16, rot=64, most=4, flags=0):
+        return lib.ffnrm_rotary(ctypes.byref(x), ctypes.byref(y), dtype, tokens, heads, dim, pos, table, rot, most, flags, None)
+
+    for kw in (dict(dtype=3), dict(dtype=-1), dict(tokens=-1), dict(dim=0), dict(rot=66), dict(rot=7), dict(rot=0), dict(most=0),
+               dict(flags=4), dict(table=None), dict(pos=None), dict(pos=18), dict(x=N.Rows(None, 64, 64)),
+               dict(y=N.Rows(64, 128, 64)), dict(x=N.Rows(65, 64, 64))):
+        assert rotary(**kw) == N.ERR_ARG, kw
+    assert rotary(tokens=0) == N.OK and rotary(heads=0) == N.OK
