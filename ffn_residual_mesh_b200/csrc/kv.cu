@@ -9,7 +9,7 @@
 #include <new>
 
 #include "kv_append.cuh"
-#include "kv_attend.cuh"
+#include "kv_attend_few.cuh"
 #include "kv_common.cuh"
 #include "kv_pages.cuh"
 #include "kv_rotary.cuh"
@@ -97,6 +97,9 @@ struct ffnrm_kv {
     float *k_scale = nullptr, *v_scale = nullptr;
     int num_sms = 148;
     int *status = nullptr;       // what kernels could not use, kStatus* bits
+    float *partial = nullptr;    // pieces of attention items cut between blocks
+    int *counters = nullptr;     // their arrivals, zero between calls
+    int few_grid[2][2] = {};     // blocks by type and row tiles
     int32_t *scratch = nullptr;  // page lists of fork / compact
     int32_t *src = nullptr, *dst = nullptr, *owner = nullptr, *list = nullptr, *rows = nullptr, *count = nullptr;
 };
@@ -147,14 +150,60 @@ void launch_append(const AppendArgs &a, bool vec, bool interleaved, unsigned gri
         append_kernel<T, false, false><<<grid, 256, 0, st>>>(a);
 }
 
-template <typename T>
-void launch_attend(const AttendArgs &a, unsigned grid, cudaStream_t st) {
-    if (a.pool.dim == 64)
-        attend_rows_kernel<T, 64><<<grid, 128, 0, st>>>(a);
-    else if (a.pool.dim == 128)
-        attend_rows_kernel<T, 128><<<grid, 128, 0, st>>>(a);
-    else
-        attend_rows_kernel<T, 256><<<grid, 128, 0, st>>>(a);
+constexpr int kFewWarps = 4, kFewMinUnits = 2;
+
+// f(kernel, dynamic shared memory, floats of one partial) of the variant for rows of type T,
+// head dim D and NT tiles of eight rows.
+template <typename F>
+int with_few(int dtype, int dim, int nt, F f) {
+#define FEW(T, D, NT) return f(attend_few_kernel<T, D, NT, kFewWarps>, few_smem<D, NT, kFewWarps>(), few_slot<D, NT>())
+#define FEW_T(T)                                                                                              \
+    switch (dim * 4 + nt) {                                                                                   \
+        case 64 * 4 + 1: FEW(T, 64, 1);                                                                       \
+        case 64 * 4 + 2: FEW(T, 64, 2);                                                                       \
+        case 128 * 4 + 1: FEW(T, 128, 1);                                                                     \
+        case 128 * 4 + 2: FEW(T, 128, 2);                                                                     \
+        case 256 * 4 + 1: FEW(T, 256, 1);                                                                     \
+        default: FEW(T, 256, 2);                                                                              \
+    }
+    if (dtype == FFNRM_F16) {
+        FEW_T(__half)
+    } else {
+        FEW_T(__nv_bfloat16)
+    }
+#undef FEW_T
+#undef FEW
+}
+
+// Prepares every variant and sizes the workspace of partials: one block per free slot of the GPU.
+int prepare_few(ffnrm_kv *kv, size_t &floats) {
+    int rc = FFNRM_OK;
+    for (int dtype : {FFNRM_F16, FFNRM_BF16})
+        for (int nt : {1, 2}) {
+            rc = with_few(dtype, kv->cfg.head_dim, nt, [&](auto kernel, int smem, int slot) {
+                int per_sm = 0;
+                KV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+                KV_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kFewWarps * 32, smem));
+                const int grid = std::max(1, per_sm) * kv->num_sms;
+                kv->few_grid[dtype][nt - 1] = grid;
+                floats = std::max(floats, size_t(2) * grid * slot);
+                return int(FFNRM_OK);
+            });
+            if (rc) return rc;
+        }
+    return rc;
+}
+
+int launch_few(ffnrm_kv *kv, const AttendArgs &a, int dtype, cudaStream_t st) {
+    // rows of one kv head that a sequence brings on average
+    const int64_t rows = int64_t(a.group) * ((a.batch.rows + a.batch.seqs - 1) / a.batch.seqs);
+    const int nt = rows > 8 ? 2 : 1;
+    const FewArgs f{a, kv->partial, kv->counters, kFewMinUnits};
+    return with_few(dtype, kv->cfg.head_dim, nt, [&](auto kernel, int smem, int) {
+        kernel<<<unsigned(kv->few_grid[dtype][nt - 1]), kFewWarps * 32, smem, st>>>(f);
+        KV_CUDA(cudaGetLastError());
+        return int(FFNRM_OK);
+    });
 }
 
 int launch_moves(ffnrm_kv *kv, const int32_t *src, const int32_t *dst, const int32_t *count, int most, cudaStream_t st) {
@@ -235,10 +284,23 @@ int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8
     DeviceGuard guard(device);
     cudaDeviceGetAttribute(&kv->num_sms, cudaDevAttrMultiProcessorCount, device);
     const size_t list = size_t(std::max(c.n_pages, c.max_seqs));
-    const size_t ints = 4 * list + 4 * size_t(c.max_seqs) + 2;
+    size_t floats = 0;
+    int rc = prepare_few(kv, floats);
+    if (rc) {
+        delete kv;
+        return rc;
+    }
+    const size_t counters = size_t(*std::max_element(&kv->few_grid[0][0], &kv->few_grid[0][0] + 4));
+    const size_t ints = 4 * list + 4 * size_t(c.max_seqs) + 2 + counters;
     const int bitmap = (c.n_pages + 31) / 32 * 4;
+    if (cudaMalloc(&kv->partial, floats * sizeof(float)) != cudaSuccess) {
+        cudaGetLastError();
+        delete kv;
+        return fail(FFNRM_ERR_NOMEM, "cudaMalloc of %zu bytes failed", floats * sizeof(float));
+    }
     if (cudaMalloc(&kv->scratch, ints * sizeof(int32_t)) != cudaSuccess) {
         cudaGetLastError();
+        cudaFree(kv->partial);
         delete kv;
         return fail(FFNRM_ERR_NOMEM, "cudaMalloc of %zu bytes failed", ints * sizeof(int32_t));
     }
@@ -249,12 +311,14 @@ int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8
     kv->rows = kv->list + list;
     kv->count = kv->rows + 4 * size_t(c.max_seqs);
     kv->status = kv->count + 1;
+    kv->counters = kv->status + 1;
     cudaError_t e = cudaMemset(kv->scratch, 0, ints * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(bitmap, 1 << 17));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(bitmap, 1 << 17));
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e != cudaSuccess) {
         cudaFree(kv->scratch);
+        cudaFree(kv->partial);
         delete kv;
         return fail(FFNRM_ERR_CUDA, "creating the cache failed: %s", cudaGetErrorString(e));
     }
@@ -266,6 +330,7 @@ int ffnrm_kv_destroy(ffnrm_kv *kv) {
     if (!kv) return FFNRM_OK;
     DeviceGuard guard(kv->device);
     cudaFree(kv->scratch);  // waits for the device
+    cudaFree(kv->partial);
     cudaGetLastError();
     delete kv;
     return FFNRM_OK;
@@ -360,16 +425,10 @@ int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     if (!aligned(lse, 4)) return fail(FFNRM_ERR_ARG, "lse must be 4-byte aligned");
     const AttendArgs a{layer_pool(kv, layer), batch_view(batch), q->data, out->data, lse, q->token_stride, q->head_stride,
                        out->token_stride, out->head_stride, q_heads / kv->cfg.kv_heads, scale, causal, window, kv->status};
-    const int64_t grid = (int64_t(batch->rows) * q_heads + 3) / 4;
-    if (grid > 0x7fffffff) return fail(FFNRM_ERR_ARG, "rows=%d are too many for one call", batch->rows);
+    if (int64_t(batch->rows) * a.group > 0x7fffffff / 2)
+        return fail(FFNRM_ERR_ARG, "rows=%d are too many for one call", batch->rows);
     DeviceGuard guard(kv->device);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == FFNRM_F16)
-        launch_attend<__half>(a, unsigned(grid), st);
-    else
-        launch_attend<__nv_bfloat16>(a, unsigned(grid), st);
-    KV_CUDA(cudaGetLastError());
-    return FFNRM_OK;
+    return launch_few(kv, a, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int ffnrm_kv_fork(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, int seqs, int table_width,
