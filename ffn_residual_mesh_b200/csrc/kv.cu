@@ -9,7 +9,7 @@
 #include <new>
 
 #include "kv_append.cuh"
-#include "kv_attend_few.cuh"
+#include "kv_attend_many.cuh"
 #include "kv_common.cuh"
 #include "kv_pages.cuh"
 #include "kv_rotary.cuh"
@@ -151,6 +151,8 @@ void launch_append(const AppendArgs &a, bool vec, bool interleaved, unsigned gri
 }
 
 constexpr int kFewWarps = 4, kFewMinUnits = 2;
+// Sequences with more query rows (tokens x group) than this take the tcgen05 kernel.
+constexpr int kFewRows = 64;
 
 // f(kernel, dynamic shared memory, floats of one partial) of the variant for rows of type T,
 // head dim D and NT tiles of eight rows.
@@ -194,16 +196,43 @@ int prepare_few(ffnrm_kv *kv, size_t &floats) {
     return rc;
 }
 
-int launch_few(ffnrm_kv *kv, const AttendArgs &a, int dtype, cudaStream_t st) {
+int launch_few(ffnrm_kv *kv, const AttendArgs &a, int dtype, int most_rows, cudaStream_t st) {
     // rows of one kv head that a sequence brings on average
     const int64_t rows = int64_t(a.group) * ((a.batch.rows + a.batch.seqs - 1) / a.batch.seqs);
     const int nt = rows > 8 ? 2 : 1;
-    const FewArgs f{a, kv->partial, kv->counters, kFewMinUnits};
+    const FewArgs f{a, kv->partial, kv->counters, kFewMinUnits, most_rows};
     return with_few(dtype, kv->cfg.head_dim, nt, [&](auto kernel, int smem, int) {
         kernel<<<unsigned(kv->few_grid[dtype][nt - 1]), kFewWarps * 32, smem, st>>>(f);
         KV_CUDA(cudaGetLastError());
         return int(FFNRM_OK);
     });
+}
+
+template <typename T, int D>
+int launch_many_t(ffnrm_kv *kv, const ManyArgs &m, cudaStream_t st) {
+    attend_many_kernel<T, D><<<unsigned(m.slots) * unsigned(kv->cfg.kv_heads), Many<D>::THREADS, Many<D>::SMEM, st>>>(m);
+    KV_CUDA(cudaGetLastError());
+    return FFNRM_OK;
+}
+
+template <typename T>
+cudaError_t prepare_many(int dim) {
+    if (dim == 64)
+        return cudaFuncSetAttribute(attend_many_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<64>::SMEM);
+    if (dim == 128)
+        return cudaFuncSetAttribute(attend_many_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<128>::SMEM);
+    return cudaFuncSetAttribute(attend_many_kernel<T, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<256>::SMEM);
+}
+
+int launch_many(ffnrm_kv *kv, const AttendArgs &a, int dtype, int few_rows, bool alone, cudaStream_t st) {
+    const int tile = kv->cfg.head_dim == 256 ? Many<256>::ROWS : Many<128>::ROWS;
+    const int64_t slots = many_slots(a.batch.seqs, a.batch.rows, a.group, tile);
+    if (slots * kv->cfg.kv_heads > 0x7fffffff) return fail(FFNRM_ERR_ARG, "rows=%d are too many for one call", a.batch.rows);
+    const ManyArgs m{a, int(slots), few_rows, alone};
+    const bool f16 = dtype == FFNRM_F16;
+    if (kv->cfg.head_dim == 64) return f16 ? launch_many_t<__half, 64>(kv, m, st) : launch_many_t<__nv_bfloat16, 64>(kv, m, st);
+    if (kv->cfg.head_dim == 128) return f16 ? launch_many_t<__half, 128>(kv, m, st) : launch_many_t<__nv_bfloat16, 128>(kv, m, st);
+    return f16 ? launch_many_t<__half, 256>(kv, m, st) : launch_many_t<__nv_bfloat16, 256>(kv, m, st);
 }
 
 int launch_moves(ffnrm_kv *kv, const int32_t *src, const int32_t *dst, const int32_t *count, int most, cudaStream_t st) {
@@ -315,6 +344,8 @@ int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8
     cudaError_t e = cudaMemset(kv->scratch, 0, ints * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(bitmap, 1 << 17));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(bitmap, 1 << 17));
+    if (e == cudaSuccess) e = prepare_many<__half>(c.head_dim);
+    if (e == cudaSuccess) e = prepare_many<__nv_bfloat16>(c.head_dim);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e != cudaSuccess) {
         cudaFree(kv->scratch);
@@ -428,7 +459,12 @@ int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     if (int64_t(batch->rows) * a.group > 0x7fffffff / 2)
         return fail(FFNRM_ERR_ARG, "rows=%d are too many for one call", batch->rows);
     DeviceGuard guard(kv->device);
-    return launch_few(kv, a, dtype, static_cast<cudaStream_t>(stream));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Without starts every sequence has one token; with them the device knows which kernel a sequence takes.
+    const bool can_be_many = batch->starts && int64_t(batch->rows) * a.group > kFewRows;
+    const bool only_many = can_be_many && batch->seqs == 1;
+    if (!only_many && (rc = launch_few(kv, a, dtype, can_be_many ? kFewRows : 0x7fffffff, st))) return rc;
+    return can_be_many ? launch_many(kv, a, dtype, only_many ? 0 : kFewRows, only_many, st) : FFNRM_OK;
 }
 
 int ffnrm_kv_fork(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, int seqs, int table_width,

@@ -73,6 +73,7 @@ struct FewArgs {
     float *partial;  // [2 * gridDim.x][rows of a tile][D + 2]
     int *counters;   // [gridDim.x], zero between calls
     int min_units;   // units that a block takes at least
+    int most_rows;   // sequences with more rows belong to the other kernel
 };
 
 // The stretch of a sequence that its rows see, in units of UK keys, and its row tiles.
@@ -80,14 +81,14 @@ struct SeqWork {
     int first, n, length, unit0, units, tiles;
 };
 template <int UK, int RT>
-__device__ __forceinline__ SeqWork seq_work(const AttendArgs &a, int s) {
+__device__ __forceinline__ SeqWork seq_work(const AttendArgs &a, int s, int most_rows) {
     SeqWork w{};
     const bool ok = seq_rows(a.batch, s, w.first, w.n) & seq_length(a.batch, s, a.pool.page_shift, w.length);
     if (!ok || (w.length > 0 && w.length < w.n)) {
         atomicOr(a.status, kStatusLength);
         w.length = 0;
     }
-    if (w.n == 0) return w;
+    if (w.n == 0 || w.n > most_rows / a.group) return w;
     const int lo = a.window > 0 ? max(0, w.length - w.n - a.window + 1) : 0;
     w.unit0 = lo / UK;
     w.units = max(1, (w.length + UK - 1) / UK - w.unit0);  // an idle slot's rows are written too
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
     for (int s0 = 0; s0 < a.batch.seqs; s0 += 32) {
         int64_t u = 0;
         if (s0 + lane < a.batch.seqs) {
-            const SeqWork w = seq_work<UK, RT>(a, s0 + lane);
+            const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
             u = int64_t(w.units) * w.tiles * pl.heads;
         }
         for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
     for (int s0 = 0; s0 < a.batch.seqs; s0 += 32) {
         int64_t u = 0;
         if (s0 + lane < a.batch.seqs) {
-            const SeqWork w = seq_work<UK, RT>(a, s0 + lane);
+            const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
             u = int64_t(w.units) * w.tiles * pl.heads;
         }
         int64_t run = u;
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
     }
 
     while (at < end && s < a.batch.seqs) {
-        const SeqWork w = seq_work<UK, RT>(a, s);
+        const SeqWork w = seq_work<UK, RT>(a, s, f.most_rows);
         const int64_t item = w.units ? (at - seq_at) / w.units : 0;
         if (w.units == 0 || item >= int64_t(w.tiles) * pl.heads) {
             seq_at += int64_t(w.units) * w.tiles * pl.heads;

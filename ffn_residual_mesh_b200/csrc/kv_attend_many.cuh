@@ -1,0 +1,455 @@
+// Attention over the 8-bit paged cache for many query rows per sequence (prompt chunks): bound by
+// the tensor cores and the exponentials, so both products run on tcgen05 and the softmax beside
+// them.
+//
+// One block holds NQ tiles of 128 rows (tokens x group of one kv head; f16, K-major, 128-byte
+// swizzle) and walks over the keys in tiles of BN. Warp roles:
+//   softmax warpgroups, one per row tile, one thread per row: read S from TMEM, write P = 2^(z-m)
+//     as f16 over it, rescale O in TMEM when the maximum moved by more than 2^8;
+//   converter warpgroup: codes from global memory to f16 K and V tiles in shared memory (exact:
+//     byte ^ 0x80 under the exponent of 1024, minus 1152), two stages each, and the tile's scales;
+//   one MMA thread: S = Q K^T (K-major operands) and O += P V (P from TMEM, V as it lies in the
+//     cache, N-major).
+// With two row tiles the tensor cores work on one while the other's softmax runs. MMAs of one
+// thread execute in order, so S of the next key tile may be written over P right behind the product
+// that reads it.
+#pragma once
+
+#include <type_traits>
+
+#include "kv_attend_few.cuh"
+#include "sm100.cuh"
+
+namespace ffnrm::kv {
+
+using namespace ffnrm::sm100;
+
+// Shared-memory matrix descriptor of an N-major tile with 128-byte swizzle: 64 channels (128 B) per
+// key row, 8-key atoms of 1024 B, `lbo` bytes between blocks of 64 channels.
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t addr, uint32_t lbo) {
+    uint64_t d = 0;
+    d |= uint64_t((addr >> 4) & 0x3FFF);
+    d |= uint64_t((lbo >> 4) & 0x3FFF) << 16;
+    d |= uint64_t(1024 >> 4) << 32;
+    d |= uint64_t(1) << 46;
+    d |= uint64_t(2) << 61;
+    return d;
+}
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
+}
+
+template <int D>
+struct Many {
+    static constexpr int NQ = D == 256 ? 1 : 2;    // row tiles of 128
+    static constexpr int BN = D == 256 ? 64 : 128; // keys per tile
+    static constexpr int SB = D == 256 ? 2 : 1;    // S buffers per row tile
+    static constexpr int ROWS = 128 * NQ;
+    static constexpr int THREADS = 128 * (NQ + 2);
+    static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = BN * D * 2;
+    static constexpr int CHUNKS = BN / 16;         // runs of keys with one scale
+    static constexpr int SMEM = 1024 + NQ * Q_BYTES + 4 * KV_BYTES + 2 * CHUNKS * 16 + 256;
+    static constexpr int O_COL = 256;              // first TMEM column of O
+    static constexpr bool REGS = D != 256;         // 512 threads: registers are moved to the softmax
+};
+
+struct ManyArgs {
+    AttendArgs a;
+    int slots;     // upper bound of row tiles per kv head
+    int few_rows;  // sequences with at most this many rows belong to the other kernel
+    int alone;     // the other kernel is not launched
+};
+
+// Row-tile slots: sequence s owns [starts[s] G / ROWS + s, starts[s+1] G / ROWS + s + 1), at least the
+// tiles that its n G rows fill.
+__host__ __device__ inline int64_t many_slots(int seqs, int rows, int group, int tile) { return int64_t(rows) * group / tile + seqs; }
+__device__ __forceinline__ int seq_of_many(const int32_t *starts, int seqs, int group, int tile, int slot) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = seqs;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int probe = lo + lane * step;
+        const unsigned m = __ballot_sync(0xffffffffu, probe < hi && int64_t(starts[probe]) * group / tile + probe <= slot);
+        const int last = m ? 31 - __clz(m) : 0;
+        lo += last * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyArgs args) {
+    using C = Many<D>;
+    constexpr int NQ = C::NQ, BN = C::BN, SB = C::SB, KB = D / 64;
+    constexpr float kLog2e = 1.4426950408889634f;
+    const AttendArgs &a = args.a;
+    const Pool &pl = a.pool;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
+    const float ninf = -__int_as_float(0x7f800000);
+
+    if (args.alone) zero_loose_rows<T>(a);
+    // This block's sequence, row tile and kv head.
+    const int h = int(blockIdx.x) % pl.heads, slot = int(blockIdx.x) / pl.heads;
+    int s = slot, nth = 0;
+    if (a.batch.starts) {
+        s = seq_of_many(a.batch.starts, a.batch.seqs, a.group, C::ROWS, slot);
+        nth = slot - int(int64_t(a.batch.starts[s]) * a.group / C::ROWS + s);
+    }
+    int first, n, length;
+    const bool ok = seq_rows(a.batch, s, first, n) & seq_length(a.batch, s, pl.page_shift, length);
+    if (!ok || (length > 0 && length < n)) {
+        if (tid == 0) atomicOr(a.status, kStatusLength);
+        length = 0;
+    }
+    const int64_t all_rows = int64_t(n) * a.group;
+    const int tiles = int((all_rows + C::ROWS - 1) / C::ROWS);
+    if (nth < 0 || nth >= tiles || n <= args.few_rows / a.group) return;
+    const int row0 = (tiles - 1 - nth) * C::ROWS;  // the longest rows first
+    const int rows = int(min(int64_t(C::ROWS), all_rows - row0)), pos0 = length - n;
+    const int token_lo = row0 / a.group, token_hi = (row0 + rows - 1) / a.group;
+    const int any_hi = a.causal ? min(length, pos0 + token_hi + 1) : length;
+    const int any_lo = a.window > 0 ? max(0, pos0 + token_lo - a.window + 1) : 0;
+    const int j0 = any_lo / BN, steps = max(0, (max(any_hi, 0) + BN - 1) / BN - j0);
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint8_t *sm_q = base, *sm_k = sm_q + NQ * C::Q_BYTES, *sm_v = sm_k + 2 * C::KV_BYTES;
+    float4 *sm_scale = reinterpret_cast<float4 *>(sm_v + 2 * C::KV_BYTES);  // [2][CHUNKS]: sk, log2 sv, 1/sv
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sm_scale + 2 * C::CHUNKS);
+    uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10,
+             *pv_done = bars + 12, *q_full = bars + 14;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 15);
+    int *err = reinterpret_cast<int *>(tmem_slot + 1);
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(k_full + i, 4);
+            mbar_init(v_full + i, 4);
+            mbar_init(k_empty + i, 1);
+            mbar_init(v_empty + i, 1);
+            mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, 4);
+            mbar_init(pv_done + i, 1);
+        }
+        mbar_init(q_full, 4 * NQ);
+        *err = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (wg < NQ) {
+        // ---- softmax: one thread per row
+        if constexpr (C::REGS) regs_inc<184>();
+        const int r = tid & 127, row = row0 + wg * 128 + r;
+        const bool live = wg * 128 + r < rows;
+        const int token = live ? row / a.group : 0, head = live ? row - token * a.group : 0;
+        const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
+        const uint32_t o_col = lane_base + C::O_COL + wg * D;
+        float qs = a.scale * kLog2e;
+        {
+            // this thread's query row, as f16 in the tile; bf16 rows are brought to [1, 2) by a power of two
+            const T *q = static_cast<const T *>(a.q) + int64_t(first + token) * a.q_token + int64_t(h * a.group + head) * a.q_head;
+            uint8_t *dst = sm_q + wg * C::Q_BYTES + r * 128;
+            float down = 1.f;
+            if constexpr (!std::is_same<T, __half>::value) {
+                float m = 0.f;
+                if (live)
+                    for (int c = 0; c < D / 8; ++c) {
+                        const Vec<T, 8> x = *reinterpret_cast<const Vec<T, 8> *>(q + c * 8);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(to_f32(x.v[i])));
+                    }
+                const int e = min(max(int(__float_as_uint(m) >> 23), 1), 253);
+                qs *= __uint_as_float(uint32_t(e) << 23);
+                down = __uint_as_float(uint32_t(254 - e) << 23);
+            }
+            for (int c = 0; c < D / 8; ++c) {
+                Vec<T, 8> x{};
+                if (live) x = *reinterpret_cast<const Vec<T, 8> *>(q + c * 8);
+                uint4 y;
+                y.x = pack_f16x2(to_f32(x.v[0]) * down, to_f32(x.v[1]) * down);
+                y.y = pack_f16x2(to_f32(x.v[2]) * down, to_f32(x.v[3]) * down);
+                y.z = pack_f16x2(to_f32(x.v[4]) * down, to_f32(x.v[5]) * down);
+                y.w = pack_f16x2(to_f32(x.v[6]) * down, to_f32(x.v[7]) * down);
+                *reinterpret_cast<uint4 *>(dst + (c / 8) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4)) = y;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        // keys that this row sees, [lo, hi); a row past the end sees everything and is not written
+        const int hi = !live ? 0x7fffffff : a.causal ? min(length, pos0 + token + 1) : length;
+        const int lo = live && a.window > 0 ? max(0, pos0 + token - a.window + 1) : 0;
+        const int warp_hi = __reduce_min_sync(0xffffffffu, hi), warp_lo = __reduce_max_sync(0xffffffffu, lo);
+        float m = ninf, l = 0.f;
+        bool good = true;
+        for (int j = 0; j < steps && good; ++j) {
+            const int st = j & 1, sb = SB == 2 ? st : wg;
+            const uint32_t s_col = lane_base + sb * BN;
+            good = mbar_wait(s_full + sb, SB == 2 ? (j >> 1) & 1 : j & 1, err, kErrWaitFull) &&
+                   mbar_wait(v_full + st, (j >> 1) & 1, err, kErrWaitFull);  // the scales come with V
+            good = __all_sync(0xffffffffu, good);
+            if (!good) break;
+            tc_fence_after();
+            uint32_t x[BN];
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) tmem_ld32(s_col + c, *reinterpret_cast<uint32_t(*)[32]>(&x[c]));
+            tmem_wait_ld();
+            const float4 *scales = sm_scale + st * C::CHUNKS;
+            const int key0 = (j0 + j) * BN;
+            const bool whole = key0 + BN <= warp_hi && key0 >= warp_lo;
+            float top = ninf;
+            if (whole) {
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) {
+                    float t = __uint_as_float(x[c]);
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) t = fmaxf(t, __uint_as_float(x[c + i]));
+                    const float4 sc = scales[c / 16];
+                    top = fmaxf(top, fmaf(t, qs * sc.x, sc.y));
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) {
+                    const float4 sc = scales[c / 16];
+                    const float f0 = qs * sc.x;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = key0 + c + i;
+                        const float z = key >= lo && key < hi ? fmaf(__uint_as_float(x[c + i]), f0, sc.y) : ninf;
+                        x[c + i] = __float_as_uint(z);
+                        top = fmaxf(top, z);
+                    }
+                }
+            }
+            const bool raise = top > m + kFewStep;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float to = raise ? top : m;
+                if (j > 0) {
+                    const float fix = raise ? (m == ninf ? 0.f : ex2(m - to)) : 1.f;
+                    l *= fix;
+                    good = __all_sync(0xffffffffu, mbar_wait(pv_done + wg, (j - 1) & 1, err, kErrWaitDone));
+                    if (!good) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_col + c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+                        tmem_st16(o_col + c, o);
+                    }
+                }
+                m = to;
+            }
+            const float off = m == ninf ? 0.f : kFewOffset - m;
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) {
+                uint32_t p[16];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float4 sc = scales[c / 16 + half];
+                    const float f0 = whole ? qs * sc.x : 1.f, f1 = (whole ? sc.y : 0.f) + off;
+                    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float p0 = ex2(fmaf(__uint_as_float(x[c + half * 16 + i]), f0, f1));
+                        const float p1 = ex2(fmaf(__uint_as_float(x[c + half * 16 + i + 1]), f0, f1));
+                        sum0 += p0;
+                        sum1 += p1;
+                        p[half * 8 + i / 2] = pack_f16x2(p0, p1);
+                    }
+                    l = fmaf(sum0 + sum1, sc.z, l);
+                }
+                tmem_st16(s_col + c / 2, p);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + sb);
+        }
+        if (steps > 0 && good) good = __all_sync(0xffffffffu, mbar_wait(pv_done + wg, (steps - 1) & 1, err, kErrWaitDone));
+        tc_fence_after();
+        const float norm = l == 0.f || !good ? 0.f : 1.f / l;
+        T *out = static_cast<T *>(a.out) + int64_t(first + token) * a.o_token + int64_t(h * a.group + head) * a.o_head;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            if (steps > 0) {
+                tmem_ld32(o_col + c, o);
+                tmem_wait_ld();
+            }
+            if (!live) continue;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+                Vec<T, 8> y;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y.v[k] = from_f32<T>(norm == 0.f ? 0.f : __uint_as_float(o[i + k]) * norm);
+                *reinterpret_cast<Vec<T, 8> *>(out + c + i) = y;
+            }
+        }
+        if (a.lse && live)
+            a.lse[int64_t(first + token) * (pl.heads * a.group) + h * a.group + head] =
+                l == 0.f ? ninf : (m - kFewOffset + lg2(l)) * 0.6931471805599453f;
+    } else if (wg == NQ) {
+        // ---- converter: warp w fills keys [w BN / 4, (w + 1) BN / 4) of every tile
+        if constexpr (C::REGS) regs_dec<96>();
+        constexpr int KEYS = BN / 4, GROUPS = KEYS / 8, RUNS = KEYS / 16;
+        const int w = warp & 3;
+        const int32_t *table = a.batch.tables + int64_t(s) * a.batch.width;
+        uint4 kr[GROUPS * KB], vr[GROUPS * KB];
+        // lane: key lane / 4 of a group of eight, 16 channels lane % 4 of a block of 64
+        auto pages_of = [&](int j, int (&page)[RUNS]) {
+#pragma unroll
+            for (int i = 0; i < RUNS; ++i) {
+                const int key = (j0 + j) * BN + w * KEYS + i * 16;
+                page[i] = -2;
+                if (j < steps && key < any_hi && key + 16 > any_lo) page[i] = table[key >> pl.page_shift];
+            }
+        };
+        auto load = [&](int j, const int (&page)[RUNS], const int8_t *codes, uint4 (&r)[GROUPS * KB]) {
+#pragma unroll
+            for (int i = 0; i < RUNS; ++i) {
+                const bool have = page[i] >= 0 && page[i] < pl.pages;
+                if (!have && page[i] != -2 && lane == 0) atomicOr(a.status, kStatusPage);
+                const int key = (j0 + j) * BN + w * KEYS + i * 16;
+                const int64_t at = ((int64_t(have ? page[i] : 0) * pl.heads + h) * pl.page_tokens + (key & (pl.page_tokens - 1))) * D;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) {
+                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                        if (have) v = __ldg(reinterpret_cast<const uint4 *>(codes + at + (g * 8 + lane / 4) * D + b * 64 + (lane & 3) * 16));
+                        r[(i * 2 + g) * KB + b] = v;
+                    }
+            }
+        };
+        auto store = [&](uint8_t *tile, const uint4 (&r)[GROUPS * KB]) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    const int row = w * KEYS + g * 8 + lane / 4, c = (lane & 3) * 2;
+                    uint8_t *dst = tile + b * (BN * 128) + row * 128;
+                    const uint4 v = r[g * KB + b];
+                    const uint32_t u[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+                    *reinterpret_cast<uint4 *>(dst + ((c ^ (row & 7)) << 4)) =
+                        make_uint4(codes_f16x2<0>(u[0]), codes_f16x2<1>(u[0]), codes_f16x2<0>(u[1]), codes_f16x2<1>(u[1]));
+                    *reinterpret_cast<uint4 *>(dst + (((c + 1) ^ (row & 7)) << 4)) =
+                        make_uint4(codes_f16x2<0>(u[2]), codes_f16x2<1>(u[2]), codes_f16x2<0>(u[3]), codes_f16x2<1>(u[3]));
+                }
+        };
+        int page[RUNS];
+        pages_of(0, page);
+        load(0, page, pl.k_codes, kr);
+        bool good = true;
+        for (int j = 0; j < steps; ++j) {
+            const int st = j & 1;
+            load(j, page, pl.v_codes, vr);
+            // the tile's scales: lane i of warp w takes run i
+            float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (lane < RUNS) {
+                int pg = page[0];
+#pragma unroll
+                for (int i = 1; i < RUNS; ++i)
+                    if (lane == i) pg = page[i];
+                if (pg >= 0 && pg < pl.pages) {
+                    const int64_t ph = int64_t(pg) * pl.heads + h;
+                    const float sv = pl.v_scale[ph];
+                    // a NaN value scale reaches the rows that see it through its logarithm
+                    sc = make_float4(pl.k_scale[ph], lg2(sv), sv == sv ? __fdividef(1.f, sv) : 0.f, 0.f);
+                }
+            }
+            int next[RUNS];
+            pages_of(j + 1, next);
+            if (j >= 2) good = __all_sync(0xffffffffu, mbar_wait(k_empty + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty));
+            if (!good) break;
+            store(sm_k + st * C::KV_BYTES, kr);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full + st);
+            if (j + 1 < steps) load(j + 1, next, pl.k_codes, kr);
+            if (j >= 2) good = __all_sync(0xffffffffu, mbar_wait(v_empty + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty));
+            if (!good) break;
+            store(sm_v + st * C::KV_BYTES, vr);
+            if (lane < RUNS) sm_scale[st * C::CHUNKS + w * RUNS + lane] = sc;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_full + st);
+#pragma unroll
+            for (int i = 0; i < RUNS; ++i) page[i] = next[i];
+        }
+    } else {
+        // ---- MMA: one thread
+        if constexpr (C::REGS) regs_dec<40>();
+        if (warp == 4 * (NQ + 1) && lane == 0 && steps > 0) {
+            constexpr uint32_t idesc_s = umma_idesc_f16_f32(128, BN), idesc_o = umma_idesc_f16_f32(128, D) | (1u << 16);
+            const uint32_t q_addr = smem_u32(sm_q), k_addr = smem_u32(sm_k), v_addr = smem_u32(sm_v);
+            auto qk = [&](int j, int q) {
+                const uint32_t d = tmem + (SB == 2 ? (j & 1) : q) * BN;
+                const uint32_t qa = q_addr + q * C::Q_BYTES, ka = k_addr + (j & 1) * C::KV_BYTES;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    umma_f16(d, umma_desc_sw128(qa + (k / 4) * (128 * 128) + (k & 3) * 32),
+                             umma_desc_sw128(ka + (k / 4) * (BN * 128) + (k & 3) * 32), idesc_s, k > 0);
+                umma_commit(s_full + (SB == 2 ? (j & 1) : q));
+            };
+            auto pv = [&](int j, int q) {
+                const uint32_t p = tmem + (SB == 2 ? (j & 1) : q) * BN, d = tmem + C::O_COL + q * D;
+                const uint32_t va = v_addr + (j & 1) * C::KV_BYTES;
+#pragma unroll
+                for (int k = 0; k < BN / 16; ++k)
+                    umma_f16_ts(d, p + k * 8, umma_desc_sw128_mn(va + k * 2048, BN * 128), idesc_o, j > 0 || k > 0);
+                umma_commit(pv_done + q);
+            };
+            bool good = mbar_wait(q_full, 0, err, kErrWaitFull) && mbar_wait(k_full, 0, err, kErrWaitFull);
+            if (good) {
+                tc_fence_after();
+                for (int q = 0; q < NQ; ++q) qk(0, q);
+                umma_commit(k_empty);
+            }
+            for (int j = 0; j < steps && good; ++j) {
+                const int st = j & 1;
+                if (SB == 2 && j + 1 < steps) {
+                    good = mbar_wait(k_full + (st ^ 1), ((j + 1) >> 1) & 1, err, kErrWaitFull);
+                    if (!good) break;
+                    tc_fence_after();
+                    qk(j + 1, 0);
+                    umma_commit(k_empty + (st ^ 1));
+                }
+                for (int q = 0; q < NQ; ++q) {
+                    const int sb = SB == 2 ? st : q;
+                    good = mbar_wait(p_full + sb, SB == 2 ? (j >> 1) & 1 : j & 1, err, kErrWaitFull) &&
+                           (q > 0 || mbar_wait(v_full + st, (j >> 1) & 1, err, kErrWaitFull));
+                    if (!good) break;
+                    tc_fence_after();
+                    pv(j, q);
+                    if (q == NQ - 1) umma_commit(v_empty + st);
+                    if (SB == 1 && j + 1 < steps) {
+                        if (q == 0) good = mbar_wait(k_full + (st ^ 1), ((j + 1) >> 1) & 1, err, kErrWaitFull);
+                        if (!good) break;
+                        tc_fence_after();
+                        qk(j + 1, q);
+                        if (q == NQ - 1) umma_commit(k_empty + (st ^ 1));
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) tmem_dealloc(tmem, 512);
+    if (tid == 0 && *err) atomicOr(a.status, kStatusWait);
+}
+
+}  // namespace ffnrm::kv
