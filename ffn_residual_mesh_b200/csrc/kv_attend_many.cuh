@@ -8,7 +8,7 @@
 //     as f16 over it, rescale O in TMEM when the maximum moved by more than 2^8;
 //   converter warpgroup: codes from global memory to f16 K and V tiles in shared memory (exact:
 //     byte ^ 0x80 under the exponent of 1024, minus 1152), two stages each, and the tile's scales;
-//   one MMA thread: S = Q K^T (K-major operands) and O += P V (P from TMEM, V as it lies in the
+//   one MMA warp: S = Q K^T (K-major operands) and O += P V (P from TMEM, V as it lies in the
 //     cache, N-major).
 // With two row tiles the tensor cores work on one while the other's softmax runs. MMAs of one
 // thread execute in order, so S of the next key tile may be written over P right behind the product
@@ -34,6 +34,12 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t addr, uint32_t l
     d |= uint64_t(1) << 46;
     d |= uint64_t(2) << 61;
     return d;
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 // D[tmem] (+)= A[tmem] * B[smem], kind::f16.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -88,7 +94,8 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
     constexpr float kLog2e = 1.4426950408889634f;
     const AttendArgs &a = args.a;
     const Pool &pl = a.pool;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0), wg = warp >> 2;  // uniform for the compiler too
     const float ninf = -__int_as_float(0x7f800000);
 
     if (args.alone) zero_loose_rows<T>(a);
@@ -143,7 +150,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     if (wg < NQ) {
         // ---- softmax: one thread per row
@@ -389,57 +396,58 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             for (int i = 0; i < RUNS; ++i) page[i] = next[i];
         }
     } else {
-        // ---- MMA: one thread
+        // ---- MMA: one warp in step, one lane issues, so that the descriptors stay in uniform
+        // registers (issued from a branch on the lane they cost 280 cycles each, not 64)
         if constexpr (C::REGS) regs_dec<40>();
-        if (warp == 4 * (NQ + 1) && lane == 0 && steps > 0) {
+        if (warp == 4 * (NQ + 1) && steps > 0) {
             constexpr uint32_t idesc_s = umma_idesc_f16_f32(128, BN), idesc_o = umma_idesc_f16_f32(128, D) | (1u << 16);
-            const uint32_t q_addr = smem_u32(sm_q), k_addr = smem_u32(sm_k), v_addr = smem_u32(sm_v);
-            auto qk = [&](int j, int q) {
-                const uint32_t d = tmem + (SB == 2 ? (j & 1) : q) * BN;
-                const uint32_t qa = q_addr + q * C::Q_BYTES, ka = k_addr + (j & 1) * C::KV_BYTES;
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                    umma_f16(d, umma_desc_sw128(qa + (k / 4) * (128 * 128) + (k & 3) * 32),
-                             umma_desc_sw128(ka + (k / 4) * (BN * 128) + (k & 3) * 32), idesc_s, k > 0);
-                umma_commit(s_full + (SB == 2 ? (j & 1) : q));
-            };
-            auto pv = [&](int j, int q) {
-                const uint32_t p = tmem + (SB == 2 ? (j & 1) : q) * BN, d = tmem + C::O_COL + q * D;
-                const uint32_t va = v_addr + (j & 1) * C::KV_BYTES;
-#pragma unroll
-                for (int k = 0; k < BN / 16; ++k)
-                    umma_f16_ts(d, p + k * 8, umma_desc_sw128_mn(va + k * 2048, BN * 128), idesc_o, j > 0 || k > 0);
-                umma_commit(pv_done + q);
-            };
-            bool good = mbar_wait(q_full, 0, err, kErrWaitFull) && mbar_wait(k_full, 0, err, kErrWaitFull);
-            if (good) {
+            const uint64_t q_desc = umma_desc_sw128(smem_u32(sm_q)), k_desc = umma_desc_sw128(smem_u32(sm_k)),
+                           v_desc = umma_desc_sw128_mn(smem_u32(sm_v), BN * 128);
+            auto wait = [&](uint64_t *bar, int parity) { return bool(__all_sync(0xffffffffu, mbar_wait(bar, parity, err, kErrWaitFull))); };
+            auto qk = [&](int j, int q, bool last) {
+                const int sb = SB == 2 ? (j & 1) : q;
+                const uint64_t qd = q_desc + (q * C::Q_BYTES >> 4), kd = k_desc + ((j & 1) * C::KV_BYTES >> 4);
                 tc_fence_after();
-                for (int q = 0; q < NQ; ++q) qk(0, q);
-                umma_commit(k_empty);
-            }
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_f16(tmem + sb * BN, qd + ((k / 4) * (128 * 128) + (k & 3) * 32 >> 4),
+                                 kd + ((k / 4) * (BN * 128) + (k & 3) * 32 >> 4), idesc_s, k > 0);
+                    umma_commit(s_full + sb);
+                    if (last) umma_commit(k_empty + (j & 1));
+                }
+                __syncwarp();
+            };
+            auto pv = [&](int j, int q, bool last) {
+                const int sb = SB == 2 ? (j & 1) : q;
+                const uint64_t vd = v_desc + ((j & 1) * C::KV_BYTES >> 4);
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < BN / 16; ++k)
+                        umma_f16_ts(tmem + C::O_COL + q * D, tmem + sb * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, j > 0 || k > 0);
+                    umma_commit(pv_done + q);
+                    if (last) umma_commit(v_empty + (j & 1));
+                }
+                __syncwarp();
+            };
+            bool good = wait(q_full, 0) && wait(k_full, 0);
+            if (good)
+                for (int q = 0; q < NQ; ++q) qk(0, q, q == NQ - 1);
             for (int j = 0; j < steps && good; ++j) {
-                const int st = j & 1;
+                const int st = j & 1, phase = (j >> 1) & 1, next = ((j + 1) >> 1) & 1;
                 if (SB == 2 && j + 1 < steps) {
-                    good = mbar_wait(k_full + (st ^ 1), ((j + 1) >> 1) & 1, err, kErrWaitFull);
-                    if (!good) break;
-                    tc_fence_after();
-                    qk(j + 1, 0);
-                    umma_commit(k_empty + (st ^ 1));
+                    if (!(good = wait(k_full + (st ^ 1), next))) break;
+                    qk(j + 1, 0, true);
                 }
                 for (int q = 0; q < NQ; ++q) {
-                    const int sb = SB == 2 ? st : q;
-                    good = mbar_wait(p_full + sb, SB == 2 ? (j >> 1) & 1 : j & 1, err, kErrWaitFull) &&
-                           (q > 0 || mbar_wait(v_full + st, (j >> 1) & 1, err, kErrWaitFull));
+                    good = wait(p_full + (SB == 2 ? st : q), SB == 2 ? phase : st) && (q > 0 || wait(v_full + st, phase));
                     if (!good) break;
-                    tc_fence_after();
-                    pv(j, q);
-                    if (q == NQ - 1) umma_commit(v_empty + st);
+                    pv(j, q, q == NQ - 1);
                     if (SB == 1 && j + 1 < steps) {
-                        if (q == 0) good = mbar_wait(k_full + (st ^ 1), ((j + 1) >> 1) & 1, err, kErrWaitFull);
+                        if (q == 0) good = wait(k_full + (st ^ 1), next);
                         if (!good) break;
-                        tc_fence_after();
-                        qk(j + 1, q);
-                        if (q == NQ - 1) umma_commit(k_empty + (st ^ 1));
+                        qk(j + 1, q, q == NQ - 1);
                     }
                 }
             }
