@@ -49,6 +49,27 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of two values on the FMA pipe: x = n + r with n the nearest integer (Cody and Waite's reduction),
+// 2^r by the minimax polynomial of degree 4 on [-1/2, 1/2] (relative error 2.6e-6), n added to the
+// exponent. Values below -125 give 2^-125.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23
+    x = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+    const float2 t = fadd2(x, magic);
+    const float2 r = fadd2(x, fadd2(magic, make_float2(-t.x, -t.y)));
+    float2 p = ffma2(r, make_float2(9.570102207e-3f, 9.570102207e-3f), make_float2(5.591786280e-2f, 5.591786280e-2f));
+    p = ffma2(p, r, make_float2(2.402474433e-1f, 2.402474433e-1f));
+    p = ffma2(p, r, make_float2(6.931217909e-1f, 6.931217909e-1f));
+    p = ffma2(p, r, make_float2(9.999992847e-1f, 9.999992847e-1f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
 template <int D>
 struct Many {
     static constexpr int NQ = D == 256 ? 1 : 2;    // row tiles of 128
@@ -217,9 +238,9 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             if (whole) {
 #pragma unroll
                 for (int c = 0; c < BN; c += 16) {
-                    float t = __uint_as_float(x[c]);
+                    float t = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 1]));
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) t = fmaxf(t, __uint_as_float(x[c + i]));
+                    for (int i = 2; i < 16; i += 2) t = max3(t, __uint_as_float(x[c + i]), __uint_as_float(x[c + i + 1]));
                     const float4 sc = scales[c / 16];
                     top = fmaxf(top, fmaf(t, qs * sc.x, sc.y));
                 }
@@ -259,32 +280,43 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                 m = to;
             }
             const float off = m == ninf ? 0.f : kFewOffset - m;
+            // two of every eight pairs take the polynomial, so that the MUFU (16 a clock for the SM, as
+            // long as both products of a tile) does not hold up the tensor cores; masked tiles need 2^-inf = 0
+            auto weights = [&](auto polynomial) {
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                uint32_t p[16];
+                for (int c = 0; c < BN; c += 32) {
+                    uint32_t p[16];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const float4 sc = scales[c / 16 + half];
-                    const float f0 = whole ? qs * sc.x : 1.f, f1 = (whole ? sc.y : 0.f) + off;
-                    float sum0 = 0.f, sum1 = 0.f;
+                    for (int half = 0; half < 2; ++half) {
+                        const float4 sc = scales[c / 16 + half];
+                        const float f0 = decltype(polynomial)::value ? qs * sc.x : 1.f, f1 = decltype(polynomial)::value ? sc.y + off : off;
+                        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float p0 = ex2(fmaf(__uint_as_float(x[c + half * 16 + i]), f0, f1));
-                        const float p1 = ex2(fmaf(__uint_as_float(x[c + half * 16 + i + 1]), f0, f1));
-                        sum0 += p0;
-                        sum1 += p1;
-                        p[half * 8 + i / 2] = pack_f16x2(p0, p1);
+                        for (int i = 0; i < 16; i += 2) {
+                            float2 z = make_float2(__uint_as_float(x[c + half * 16 + i]), __uint_as_float(x[c + half * 16 + i + 1]));
+                            z = ffma2(z, make_float2(f0, f0), make_float2(f1, f1));
+                            const float2 e = decltype(polynomial)::value && (i & 7) == 6 ? ex2_poly(z) : make_float2(ex2(z.x), ex2(z.y));
+                            sum = i == 0 ? e : fadd2(sum, e);
+                            p[half * 8 + i / 2] = pack_f16x2(e.x, e.y);
+                        }
+                        l = fmaf(sum.x + sum.y, sc.z, l);
                     }
-                    l = fmaf(sum0 + sum1, sc.z, l);
+                    tmem_st16(s_col + c / 2, p);
                 }
-                tmem_st16(s_col + c / 2, p);
-            }
+            };
+            if (whole)
+                weights(std::true_type{});
+            else
+                weights(std::false_type{});
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + sb);
         }
-        if (steps > 0 && good) good = __all_sync(0xffffffffu, mbar_wait(pv_done + wg, (steps - 1) & 1, err, kErrWaitDone));
+        // The last S tells that the products up to PV(steps - 2) (two S buffers: PV(steps - 3)) are done; a
+        // parity wait may look one phase ahead only.
+        for (int j = max(0, steps - SB); j < steps && good; ++j)
+            good = __all_sync(0xffffffffu, mbar_wait(pv_done + wg, j & 1, err, kErrWaitDone));
         tc_fence_after();
         const float norm = l == 0.f || !good ? 0.f : 1.f / l;
         T *out = static_cast<T *>(a.out) + int64_t(first + token) * a.o_token + int64_t(h * a.group + head) * a.o_head;
