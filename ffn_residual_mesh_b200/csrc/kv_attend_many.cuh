@@ -35,6 +35,22 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t addr, uint32_t l
     d |= uint64_t(2) << 61;
     return d;
 }
+// Waits for the phase of `parity`, asleep in hardware for up to about 10 us at a time (the polls of
+// nine waiting warps would take a fifth of the issue slots from the softmax); gives up after some
+// seconds.
+__device__ __forceinline__ bool wait_phase(uint64_t *bar, uint32_t parity, int *err, int code) {
+    for (int i = 0; i < 400000; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(10000u)
+            : "memory");
+        if (ok) return true;
+    }
+    atomicExch(err, code);
+    return false;
+}
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -61,7 +77,8 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
     const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23
     x = make_float2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
     const float2 t = fadd2(x, magic);
-    const float2 r = fadd2(x, fadd2(magic, make_float2(-t.x, -t.y)));
+    const float2 n = fadd2(t, make_float2(-12582912.f, -12582912.f));
+    const float2 r = ffma2(n, make_float2(-1.f, -1.f), x);
     float2 p = ffma2(r, make_float2(9.570102207e-3f, 9.570102207e-3f), make_float2(5.591786280e-2f, 5.591786280e-2f));
     p = ffma2(p, r, make_float2(2.402474433e-1f, 2.402474433e-1f));
     p = ffma2(p, r, make_float2(6.931217909e-1f, 6.931217909e-1f));
@@ -80,6 +97,7 @@ struct Many {
     static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = BN * D * 2;
     static constexpr int CHUNKS = BN / 16;         // runs of keys with one scale
     static constexpr int SMEM = 1024 + NQ * Q_BYTES + 4 * KV_BYTES + 2 * CHUNKS * 16 + 256;
+    static constexpr int EARLY = BN / 4 * 3 / 32 * 32;  // keys of P that are handed over first
     static constexpr int O_COL = 256;              // first TMEM column of O
     static constexpr bool REGS = D != 256;         // 512 threads: registers are moved to the softmax
 };
@@ -149,8 +167,8 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
     float4 *sm_scale = reinterpret_cast<float4 *>(sm_v + 2 * C::KV_BYTES);  // [2][CHUNKS]: sk, log2 sv, 1/sv
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm_scale + 2 * C::CHUNKS);
     uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10,
-             *pv_done = bars + 12, *q_full = bars + 14;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 15);
+             *pv_done = bars + 12, *p_early = bars + 14, *q_full = bars + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
     int *err = reinterpret_cast<int *>(tmem_slot + 1);
 
     if (tid == 0) {
@@ -161,6 +179,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             mbar_init(v_empty + i, 1);
             mbar_init(s_full + i, 1);
             mbar_init(p_full + i, 4);
+            mbar_init(p_early + i, 4);
             mbar_init(pv_done + i, 1);
         }
         mbar_init(q_full, 4 * NQ);
@@ -183,31 +202,37 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
         const uint32_t o_col = lane_base + C::O_COL + wg * D;
         float qs = a.scale * kLog2e;
         {
-            // this thread's query row, as f16 in the tile; bf16 rows are brought to [1, 2) by a power of two
-            const T *q = static_cast<const T *>(a.q) + int64_t(first + token) * a.q_token + int64_t(h * a.group + head) * a.q_head;
-            uint8_t *dst = sm_q + wg * C::Q_BYTES + r * 128;
-            float down = 1.f;
-            if constexpr (!std::is_same<T, __half>::value) {
-                float m = 0.f;
-                if (live)
-                    for (int c = 0; c < D / 8; ++c) {
-                        const Vec<T, 8> x = *reinterpret_cast<const Vec<T, 8> *>(q + c * 8);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(to_f32(x.v[i])));
-                    }
-                const int e = min(max(int(__float_as_uint(m) >> 23), 1), 253);
-                qs *= __uint_as_float(uint32_t(e) << 23);
-                down = __uint_as_float(uint32_t(254 - e) << 23);
-            }
-            for (int c = 0; c < D / 8; ++c) {
+            // the warp's 32 query rows as f16 in the tile, D / 8 lanes to a row; bf16 rows are brought to
+            // [1, 2) by a power of two
+            constexpr int LANES = D / 8, PASS = 32 / LANES;  // rows of one load
+            const int64_t mine = int64_t(first + token) * a.q_token + int64_t(h * a.group + head) * a.q_head;
+            const int alive = __popc(__ballot_sync(0xffffffffu, live));
+            const int c = lane % LANES;
+            uint8_t *tile = sm_q + wg * C::Q_BYTES + (c / 8) * (128 * 128);
+#pragma unroll 8
+            for (int i = 0; i < 32; i += PASS) {
+                const int from = i + lane / LANES, rr = (warp & 3) * 32 + from;
+                const int64_t at = __shfl_sync(0xffffffffu, mine, from);
                 Vec<T, 8> x{};
-                if (live) x = *reinterpret_cast<const Vec<T, 8> *>(q + c * 8);
-                uint4 y;
-                y.x = pack_f16x2(to_f32(x.v[0]) * down, to_f32(x.v[1]) * down);
-                y.y = pack_f16x2(to_f32(x.v[2]) * down, to_f32(x.v[3]) * down);
-                y.z = pack_f16x2(to_f32(x.v[4]) * down, to_f32(x.v[5]) * down);
-                y.w = pack_f16x2(to_f32(x.v[6]) * down, to_f32(x.v[7]) * down);
-                *reinterpret_cast<uint4 *>(dst + (c / 8) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4)) = y;
+                if (from < alive) x = *reinterpret_cast<const Vec<T, 8> *>(static_cast<const T *>(a.q) + at + c * 8);
+                float f[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) f[k] = to_f32(x.v[k]);
+                if constexpr (!std::is_same<T, __half>::value) {
+                    float m = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
+#pragma unroll
+                    for (int o = LANES / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    const int e = min(max(int(__float_as_uint(m) >> 23), 1), 253);
+                    const float down = __uint_as_float(uint32_t(254 - e) << 23);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) f[k] *= down;
+                    const int my_e = __shfl_sync(0xffffffffu, e, (lane - i) * LANES & 31);
+                    if (lane >= i && lane < i + PASS) qs *= __uint_as_float(uint32_t(my_e) << 23);
+                }
+                *reinterpret_cast<uint4 *>(tile + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) =
+                    make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -222,8 +247,8 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
         for (int j = 0; j < steps && good; ++j) {
             const int st = j & 1, sb = SB == 2 ? st : wg;
             const uint32_t s_col = lane_base + sb * BN;
-            good = mbar_wait(s_full + sb, SB == 2 ? (j >> 1) & 1 : j & 1, err, kErrWaitFull) &&
-                   mbar_wait(v_full + st, (j >> 1) & 1, err, kErrWaitFull);  // the scales come with V
+            good = wait_phase(s_full + sb, SB == 2 ? (j >> 1) & 1 : j & 1, err, kErrWaitFull) &&
+                   wait_phase(v_full + st, (j >> 1) & 1, err, kErrWaitFull);  // the scales come with V
             good = __all_sync(0xffffffffu, good);
             if (!good) break;
             tc_fence_after();
@@ -264,7 +289,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                 if (j > 0) {
                     const float fix = raise ? (m == ninf ? 0.f : ex2(m - to)) : 1.f;
                     l *= fix;
-                    good = __all_sync(0xffffffffu, mbar_wait(pv_done + wg, (j - 1) & 1, err, kErrWaitDone));
+                    good = __all_sync(0xffffffffu, wait_phase(pv_done + wg, (j - 1) & 1, err, kErrWaitDone));
                     if (!good) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -302,6 +327,12 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                         l = fmaf(sum.x + sum.y, sc.z, l);
                     }
                     tmem_st16(s_col + c / 2, p);
+                    if (c + 32 == C::EARLY) {  // the product may begin on these keys
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_early + sb);
+                    }
                 }
             };
             if (whole)
@@ -316,7 +347,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
         // The last S tells that the products up to PV(steps - 2) (two S buffers: PV(steps - 3)) are done; a
         // parity wait may look one phase ahead only.
         for (int j = max(0, steps - SB); j < steps && good; ++j)
-            good = __all_sync(0xffffffffu, mbar_wait(pv_done + wg, j & 1, err, kErrWaitDone));
+            good = __all_sync(0xffffffffu, wait_phase(pv_done + wg, j & 1, err, kErrWaitDone));
         tc_fence_after();
         const float norm = l == 0.f || !good ? 0.f : 1.f / l;
         T *out = static_cast<T *>(a.out) + int64_t(first + token) * a.o_token + int64_t(h * a.group + head) * a.o_head;
@@ -387,45 +418,48 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                         make_uint4(codes_f16x2<0>(u[2]), codes_f16x2<1>(u[2]), codes_f16x2<0>(u[3]), codes_f16x2<1>(u[3]));
                 }
         };
-        int page[RUNS];
+        // the scales of run `lane` of a tile: loaded a tile ahead, as the page ids are two ahead
+        float2 sc = make_float2(0.f, 1.f);
+        auto load_scales = [&](const int (&page)[RUNS]) {
+            sc = make_float2(0.f, 1.f);
+            if (lane >= RUNS) return;
+            int pg = page[0];
+#pragma unroll
+            for (int i = 1; i < RUNS; ++i)
+                if (lane == i) pg = page[i];
+            if (pg < 0 || pg >= pl.pages) return;
+            const int64_t ph = int64_t(pg) * pl.heads + h;
+            sc = make_float2(pl.k_scale[ph], pl.v_scale[ph]);
+        };
+        int page[RUNS], next[RUNS];
         pages_of(0, page);
+        pages_of(1, next);
         load(0, page, pl.k_codes, kr);
+        load_scales(page);
         bool good = true;
         for (int j = 0; j < steps; ++j) {
             const int st = j & 1;
             load(j, page, pl.v_codes, vr);
-            // the tile's scales: lane i of warp w takes run i
-            float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (lane < RUNS) {
-                int pg = page[0];
 #pragma unroll
-                for (int i = 1; i < RUNS; ++i)
-                    if (lane == i) pg = page[i];
-                if (pg >= 0 && pg < pl.pages) {
-                    const int64_t ph = int64_t(pg) * pl.heads + h;
-                    const float sv = pl.v_scale[ph];
-                    // a NaN value scale reaches the rows that see it through its logarithm
-                    sc = make_float4(pl.k_scale[ph], lg2(sv), sv == sv ? __fdividef(1.f, sv) : 0.f, 0.f);
-                }
-            }
-            int next[RUNS];
-            pages_of(j + 1, next);
-            if (j >= 2) good = __all_sync(0xffffffffu, mbar_wait(k_empty + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty));
+            for (int i = 0; i < RUNS; ++i) page[i] = next[i];
+            pages_of(j + 2, next);
+            if (j >= 2) good = __all_sync(0xffffffffu, wait_phase(k_empty + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty));
             if (!good) break;
             store(sm_k + st * C::KV_BYTES, kr);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(k_full + st);
-            if (j + 1 < steps) load(j + 1, next, pl.k_codes, kr);
-            if (j >= 2) good = __all_sync(0xffffffffu, mbar_wait(v_empty + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty));
+            if (j + 1 < steps) load(j + 1, page, pl.k_codes, kr);
+            if (j >= 2) good = __all_sync(0xffffffffu, wait_phase(v_empty + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty));
             if (!good) break;
+            // a NaN value scale reaches the rows that see it through its logarithm
+            if (lane < RUNS)
+                sm_scale[st * C::CHUNKS + w * RUNS + lane] = make_float4(sc.x, lg2(sc.y), sc.y == sc.y ? __fdividef(1.f, sc.y) : 0.f, 0.f);
+            if (j + 1 < steps) load_scales(page);
             store(sm_v + st * C::KV_BYTES, vr);
-            if (lane < RUNS) sm_scale[st * C::CHUNKS + w * RUNS + lane] = sc;
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(v_full + st);
-#pragma unroll
-            for (int i = 0; i < RUNS; ++i) page[i] = next[i];
         }
     } else {
         // ---- MMA: one warp in step, one lane issues, so that the descriptors stay in uniform
@@ -435,7 +469,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             constexpr uint32_t idesc_s = umma_idesc_f16_f32(128, BN), idesc_o = umma_idesc_f16_f32(128, D) | (1u << 16);
             const uint64_t q_desc = umma_desc_sw128(smem_u32(sm_q)), k_desc = umma_desc_sw128(smem_u32(sm_k)),
                            v_desc = umma_desc_sw128_mn(smem_u32(sm_v), BN * 128);
-            auto wait = [&](uint64_t *bar, int parity) { return bool(__all_sync(0xffffffffu, mbar_wait(bar, parity, err, kErrWaitFull))); };
+            auto wait = [&](uint64_t *bar, int parity) { return bool(__all_sync(0xffffffffu, wait_phase(bar, parity, err, kErrWaitFull))); };
             auto qk = [&](int j, int q, bool last) {
                 const int sb = SB == 2 ? (j & 1) : q;
                 const uint64_t qd = q_desc + (q * C::Q_BYTES >> 4), kd = k_desc + ((j & 1) * C::KV_BYTES >> 4);
@@ -451,31 +485,39 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                 __syncwarp();
             };
             auto pv = [&](int j, int q, bool last) {
-                const int sb = SB == 2 ? (j & 1) : q;
+                const int sb = SB == 2 ? (j & 1) : q, turn = SB == 2 ? (j >> 1) & 1 : j & 1;
                 const uint64_t vd = v_desc + ((j & 1) * C::KV_BYTES >> 4);
-                tc_fence_after();
-                if (elect_one()) {
+                auto keys = [&](int k0, int k1) {
+                    tc_fence_after();
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < BN / 16; ++k)
-                        umma_f16_ts(tmem + C::O_COL + q * D, tmem + sb * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, j > 0 || k > 0);
-                    umma_commit(pv_done + q);
-                    if (last) umma_commit(v_empty + (j & 1));
-                }
-                __syncwarp();
+                        for (int k = 0; k < BN / 16; ++k)
+                            if (k >= k0 && k < k1)
+                                umma_f16_ts(tmem + C::O_COL + q * D, tmem + sb * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, j > 0 || k > 0);
+                        if (k1 == BN / 16) {
+                            umma_commit(pv_done + q);
+                            if (last) umma_commit(v_empty + (j & 1));
+                        }
+                    }
+                    __syncwarp();
+                };
+                if (!wait(p_early + sb, turn) || (q == 0 && !wait(v_full + (j & 1), (j >> 1) & 1))) return false;
+                keys(0, C::EARLY / 16);
+                if (!wait(p_full + sb, turn)) return false;
+                keys(C::EARLY / 16, BN / 16);
+                return true;
             };
             bool good = wait(q_full, 0) && wait(k_full, 0);
             if (good)
                 for (int q = 0; q < NQ; ++q) qk(0, q, q == NQ - 1);
             for (int j = 0; j < steps && good; ++j) {
-                const int st = j & 1, phase = (j >> 1) & 1, next = ((j + 1) >> 1) & 1;
+                const int st = j & 1, next = ((j + 1) >> 1) & 1;
                 if (SB == 2 && j + 1 < steps) {
                     if (!(good = wait(k_full + (st ^ 1), next))) break;
                     qk(j + 1, 0, true);
                 }
                 for (int q = 0; q < NQ; ++q) {
-                    good = wait(p_full + (SB == 2 ? st : q), SB == 2 ? phase : st) && (q > 0 || wait(v_full + st, phase));
-                    if (!good) break;
-                    pv(j, q, q == NQ - 1);
+                    if (!(good = pv(j, q, q == NQ - 1))) break;
                     if (SB == 1 && j + 1 < steps) {
                         if (q == 0) good = wait(k_full + (st ^ 1), next);
                         if (!good) break;
