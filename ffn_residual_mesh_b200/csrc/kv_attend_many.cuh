@@ -93,7 +93,8 @@ struct Many {
     static constexpr int BN = D == 256 ? 64 : 128; // keys per tile
     static constexpr int SB = D == 256 ? 2 : 1;    // S buffers per row tile
     static constexpr int ROWS = 128 * NQ;
-    static constexpr int THREADS = 128 * (NQ + 2);
+    static constexpr int CONV = D == 256 ? 2 : 1;  // converter warpgroups
+    static constexpr int THREADS = 128 * (NQ + CONV + 1);
     static constexpr int Q_BYTES = 128 * D * 2, KV_BYTES = BN * D * 2;
     static constexpr int CHUNKS = BN / 16;         // runs of keys with one scale
     static constexpr int SMEM = 1024 + NQ * Q_BYTES + 4 * KV_BYTES + 2 * CHUNKS * 16 + 256;
@@ -167,8 +168,8 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
     float4 *sm_scale = reinterpret_cast<float4 *>(sm_v + 2 * C::KV_BYTES);  // [2][CHUNKS]: sk, log2 sv, 1/sv
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm_scale + 2 * C::CHUNKS);
     uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10,
-             *pv_done = bars + 12, *p_early = bars + 14, *q_full = bars + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
+             *pv_done = bars + 12, *p_early = bars + 14, *q_full = bars + 16, *o_full = bars + 17;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 19);
     int *err = reinterpret_cast<int *>(tmem_slot + 1);
 
     if (tid == 0) {
@@ -181,6 +182,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             mbar_init(p_full + i, 4);
             mbar_init(p_early + i, 4);
             mbar_init(pv_done + i, 1);
+            mbar_init(o_full + i, 1);
         }
         mbar_init(q_full, 4 * NQ);
         *err = 0;
@@ -344,10 +346,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + sb);
         }
-        // The last S tells that the products up to PV(steps - 2) (two S buffers: PV(steps - 3)) are done; a
-        // parity wait may look one phase ahead only.
-        for (int j = max(0, steps - SB); j < steps && good; ++j)
-            good = __all_sync(0xffffffffu, wait_phase(pv_done + wg, j & 1, err, kErrWaitDone));
+        if (steps > 0 && good) good = __all_sync(0xffffffffu, wait_phase(o_full + wg, 0, err, kErrWaitDone));
         tc_fence_after();
         const float norm = l == 0.f || !good ? 0.f : 1.f / l;
         T *out = static_cast<T *>(a.out) + int64_t(first + token) * a.o_token + int64_t(h * a.group + head) * a.o_head;
@@ -370,13 +369,13 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
         if (a.lse && live)
             a.lse[int64_t(first + token) * (pl.heads * a.group) + h * a.group + head] =
                 l == 0.f ? ninf : (m - kFewOffset + lg2(l)) * 0.6931471805599453f;
-    } else if (wg == NQ) {
-        // ---- converter: warp w fills keys [w BN / 4, (w + 1) BN / 4) of every tile
+    } else if (wg < NQ + C::CONV) {
+        // ---- converters: warp w fills keys [w BN / 4, (w + 1) BN / 4) of every tile
         if constexpr (C::REGS) regs_dec<96>();
         constexpr int KEYS = BN / 4, GROUPS = KEYS / 8, RUNS = KEYS / 16;
         const int w = warp & 3;
         const int32_t *table = a.batch.tables + int64_t(s) * a.batch.width;
-        uint4 kr[GROUPS * KB], vr[GROUPS * KB];
+        uint4 kr[GROUPS * KB];
         // lane: key lane / 4 of a group of eight, 16 channels lane % 4 of a block of 64
         auto pages_of = [&](int j, int (&page)[RUNS]) {
 #pragma unroll
@@ -431,46 +430,64 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             const int64_t ph = int64_t(pg) * pl.heads + h;
             sc = make_float2(pl.k_scale[ph], pl.v_scale[ph]);
         };
+        auto fill = [&](bool v, int j, const uint4 (&r)[GROUPS * KB]) {  // wait for the stage, convert, hand over
+            const int st = j & 1;
+            if (j >= 2 && !__all_sync(0xffffffffu, wait_phase((v ? v_empty : k_empty) + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty))) return false;
+            // a NaN value scale reaches the rows that see it through its logarithm
+            if (v && lane < RUNS)
+                sm_scale[st * C::CHUNKS + w * RUNS + lane] = make_float4(sc.x, lg2(sc.y), sc.y == sc.y ? __fdividef(1.f, sc.y) : 0.f, 0.f);
+            store((v ? sm_v : sm_k) + st * C::KV_BYTES, r);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive((v ? v_full : k_full) + st);
+            return true;
+        };
         int page[RUNS], next[RUNS];
         pages_of(0, page);
         pages_of(1, next);
-        load(0, page, pl.k_codes, kr);
-        load_scales(page);
-        bool good = true;
-        for (int j = 0; j < steps; ++j) {
-            const int st = j & 1;
-            load(j, page, pl.v_codes, vr);
+        if constexpr (C::CONV == 2) {
+            // one warpgroup for K, one for V
+            const bool v = wg == NQ + 1;
+            const int8_t *codes = v ? pl.v_codes : pl.k_codes;
+            load(0, page, codes, kr);
+            load_scales(page);
+            for (int j = 0; j < steps; ++j) {
+                if (!fill(v, j, kr)) break;
+                if (j + 1 < steps) {
+                    load(j + 1, next, codes, kr);
+                    load_scales(next);
+                    pages_of(j + 2, next);
+                }
+            }
+        } else {
+            uint4 vr[GROUPS * KB];
+            load(0, page, pl.k_codes, kr);
+            load_scales(page);
+            for (int j = 0; j < steps; ++j) {
+                load(j, page, pl.v_codes, vr);
 #pragma unroll
-            for (int i = 0; i < RUNS; ++i) page[i] = next[i];
-            pages_of(j + 2, next);
-            if (j >= 2) good = __all_sync(0xffffffffu, wait_phase(k_empty + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty));
-            if (!good) break;
-            store(sm_k + st * C::KV_BYTES, kr);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(k_full + st);
-            if (j + 1 < steps) load(j + 1, page, pl.k_codes, kr);
-            if (j >= 2) good = __all_sync(0xffffffffu, wait_phase(v_empty + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty));
-            if (!good) break;
-            // a NaN value scale reaches the rows that see it through its logarithm
-            if (lane < RUNS)
-                sm_scale[st * C::CHUNKS + w * RUNS + lane] = make_float4(sc.x, lg2(sc.y), sc.y == sc.y ? __fdividef(1.f, sc.y) : 0.f, 0.f);
-            if (j + 1 < steps) load_scales(page);
-            store(sm_v + st * C::KV_BYTES, vr);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(v_full + st);
+                for (int i = 0; i < RUNS; ++i) page[i] = next[i];
+                pages_of(j + 2, next);
+                if (!fill(false, j, kr)) break;
+                if (j + 1 < steps) load(j + 1, page, pl.k_codes, kr);
+                if (!fill(true, j, vr)) break;
+                if (j + 1 < steps) load_scales(page);
+            }
         }
     } else {
         // ---- MMA: one warp in step, one lane issues, so that the descriptors stay in uniform
-        // registers (issued from a branch on the lane they cost 280 cycles each, not 64)
+        // registers (issued from a branch on the lane they cost 280 cycles each, not 64); a warp for
+        // each row tile, whose products then mix, was a tenth slower
         if constexpr (C::REGS) regs_dec<40>();
-        if (warp == 4 * (NQ + 1) && steps > 0) {
+        if (warp == 4 * (NQ + C::CONV) && steps > 0) {
             constexpr uint32_t idesc_s = umma_idesc_f16_f32(128, BN), idesc_o = umma_idesc_f16_f32(128, D) | (1u << 16);
             const uint64_t q_desc = umma_desc_sw128(smem_u32(sm_q)), k_desc = umma_desc_sw128(smem_u32(sm_k)),
                            v_desc = umma_desc_sw128_mn(smem_u32(sm_v), BN * 128);
-            auto wait = [&](uint64_t *bar, int parity) { return bool(__all_sync(0xffffffffu, wait_phase(bar, parity, err, kErrWaitFull))); };
-            auto qk = [&](int j, int q, bool last) {
+            auto wait = [&](uint64_t *bar, int parity) {
+                const bool done = wait_phase(bar, parity, err, kErrWaitFull);
+                return bool(__all_sync(0xffffffffu, done));
+            };
+            auto qk = [&](int j, int q) {
                 const int sb = SB == 2 ? (j & 1) : q;
                 const uint64_t qd = q_desc + (q * C::Q_BYTES >> 4), kd = k_desc + ((j & 1) * C::KV_BYTES >> 4);
                 tc_fence_after();
@@ -480,49 +497,43 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                         umma_f16(tmem + sb * BN, qd + ((k / 4) * (128 * 128) + (k & 3) * 32 >> 4),
                                  kd + ((k / 4) * (BN * 128) + (k & 3) * 32 >> 4), idesc_s, k > 0);
                     umma_commit(s_full + sb);
-                    if (last) umma_commit(k_empty + (j & 1));
+                    if (q == NQ - 1) umma_commit(k_empty + (j & 1));
                 }
                 __syncwarp();
             };
-            auto pv = [&](int j, int q, bool last) {
-                const int sb = SB == 2 ? (j & 1) : q, turn = SB == 2 ? (j >> 1) & 1 : j & 1;
+            auto pv = [&](int j, int q, int k0, int k1) {  // 16-key steps k0 .. k1 - 1
+                const int sb = SB == 2 ? (j & 1) : q;
                 const uint64_t vd = v_desc + ((j & 1) * C::KV_BYTES >> 4);
-                auto keys = [&](int k0, int k1) {
-                    tc_fence_after();
-                    if (elect_one()) {
+                tc_fence_after();
+                if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < BN / 16; ++k)
-                            if (k >= k0 && k < k1)
-                                umma_f16_ts(tmem + C::O_COL + q * D, tmem + sb * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, j > 0 || k > 0);
-                        if (k1 == BN / 16) {
-                            umma_commit(pv_done + q);
-                            if (last) umma_commit(v_empty + (j & 1));
-                        }
+                    for (int k = 0; k < BN / 16; ++k)
+                        if (k >= k0 && k < k1)
+                            umma_f16_ts(tmem + C::O_COL + q * D, tmem + sb * BN + k * 8, vd + (k * 2048 >> 4), idesc_o, j > 0 || k > 0);
+                    if (k1 == BN / 16) {
+                        umma_commit(pv_done + q);
+                        if (q == NQ - 1) umma_commit(v_empty + (j & 1));
+                        if (j + 1 == steps) umma_commit(o_full + q);
                     }
-                    __syncwarp();
-                };
-                if (!wait(p_early + sb, turn) || (q == 0 && !wait(v_full + (j & 1), (j >> 1) & 1))) return false;
-                keys(0, C::EARLY / 16);
-                if (!wait(p_full + sb, turn)) return false;
-                keys(C::EARLY / 16, BN / 16);
-                return true;
+                }
+                __syncwarp();
             };
             bool good = wait(q_full, 0) && wait(k_full, 0);
-            if (good)
-                for (int q = 0; q < NQ; ++q) qk(0, q, q == NQ - 1);
+            for (int q = 0; q < NQ && good; ++q) qk(0, q);
             for (int j = 0; j < steps && good; ++j) {
-                const int st = j & 1, next = ((j + 1) >> 1) & 1;
+                const int st = j & 1, phase = (j >> 1) & 1, next = ((j + 1) >> 1) & 1;
                 if (SB == 2 && j + 1 < steps) {
                     if (!(good = wait(k_full + (st ^ 1), next))) break;
-                    qk(j + 1, 0, true);
+                    qk(j + 1, 0);
                 }
                 for (int q = 0; q < NQ; ++q) {
-                    if (!(good = pv(j, q, q == NQ - 1))) break;
-                    if (SB == 1 && j + 1 < steps) {
-                        if (q == 0) good = wait(k_full + (st ^ 1), next);
-                        if (!good) break;
-                        qk(j + 1, q, q == NQ - 1);
-                    }
+                    const int sb = SB == 2 ? st : q, turn = SB == 2 ? phase : st;
+                    if (!(good = (q > 0 || wait(v_full + st, phase)) && wait(p_early + sb, turn))) break;
+                    pv(j, q, 0, C::EARLY / 16);
+                    if (SB == 1 && j + 1 < steps && q == 0 && !(good = wait(k_full + (st ^ 1), next))) break;
+                    if (!(good = wait(p_full + sb, turn))) break;
+                    pv(j, q, C::EARLY / 16, BN / 16);
+                    if (SB == 1 && j + 1 < steps) qk(j + 1, q);
                 }
             }
         }
