@@ -11,6 +11,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libffnrm.so"
+BIND_PATH = LIB_PATH.parent / "ffnrm_kv_bind.so"  # Python binding of the paged cache's calls
 
 OK, ERR_ARG, ERR_CUDA, ERR_STATE, ERR_NOMEM, ERR_TIMEOUT = 0, 1, 2, 3, 4, 5
 CODES_Q4_BYTES, CODES_QLO2_ROWPACKED, CODES_BITPLANES = 0, 1, 2
@@ -89,6 +90,11 @@ class LayerWeights(ctypes.Structure):
 class KvConfig(ctypes.Structure):
     _fields_ = [("n_layers", c_int32), ("n_pages", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
                 ("page_tokens", c_int32), ("max_seqs", c_int32)]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("tables", c_void_p), ("lengths", c_void_p), ("starts", c_void_p), ("seqs", c_int32),
+                ("table_width", c_int32), ("rows", c_int32)]
 
 
 class KvBatch(ctypes.Structure):

@@ -63,6 +63,25 @@ def included(source: Path) -> list[Path]:
     return found
 
 
+# Python binding of the paged cache's calls (torch tensors in, C ABI out).
+BIND_SOURCE = CSRC / "kv_bind.cpp"
+BIND = LIB_DIR / "ffnrm_kv_bind.so"
+
+
+def bind_command() -> list[str]:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    cuda = Path(nvcc()).resolve().parent.parent
+    libs = Path(torch.__file__).resolve().parent / "lib"
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-isystem{p}" for p in cpp_extension.include_paths()), f"-isystem{sysconfig.get_paths()['include']}",
+            f"-isystem{cuda / 'include'}", *INCLUDES, str(BIND_SOURCE), "-o", str(BIND), f"-L{LIB_DIR}", "-lffnrm", f"-L{libs}",
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
+
+
 # Drop-in runner executables (same argv / exit codes / JSON as the reference's runners),
 # host C++ over the C ABI; they find libffnrm.so through an $ORIGIN-relative rpath.
 HOST = PKG / "host"
@@ -109,6 +128,11 @@ def build(force: bool = False, verbose: bool = False, runners: bool = True) -> P
             for done in pool.map(subprocess.run, todo):
                 done.check_returncode()
         subprocess.run(link_command(), check=True)
+    if force or stale(BIND, [BIND_SOURCE, ROOT / "include" / "ffnrm.h"]):
+        cmd = bind_command()
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        subprocess.run(cmd, check=True)
     if runners:
         build_runners(force, verbose)
     return LIB

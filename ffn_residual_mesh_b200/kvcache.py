@@ -27,40 +27,23 @@ from . import _native as N
 from .engine import _stream
 
 
-def _dtype(x) -> int:
-    import torch
-    try:
-        return {torch.float16: N.F16, torch.bfloat16: N.BF16, torch.float32: N.F32}[x.dtype]
-    except KeyError:
-        raise ValueError(f"expected float16, bfloat16 or float32, got {x.dtype}") from None
+_module = None
 
 
-def _on(name, x, device):
-    if x.device != device:
-        raise ValueError(f"{name} must be on {device}, got {x.device}")
+def _bind():
+    """The compiled binding of the cache's calls (built with the library)."""
+    global _module
+    if _module is None:
+        import importlib.util
 
-
-def _rows(name, x, heads, dim, rows=None) -> N.Rows:
-    """A [rows, heads, dim] view with contiguous channels."""
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != dim or (rows is not None and x.shape[0] != rows):
-        raise ValueError(f"{name} must have shape ({'T' if rows is None else rows}, {heads}, {dim}), got {tuple(x.shape)}")
-    if x.stride(2) != 1 and dim > 1 and x.numel():
-        raise ValueError(f"{name} must have contiguous channels")
-    return N.Rows(x.data_ptr(), x.stride(0), x.stride(1))
-
-
-def _writable(name, x):
-    """A tensor that is written must not name one element twice (an expanded view)."""
-    if any(st == 0 and n > 1 for st, n in zip(x.stride(), x.shape)):
-        raise ValueError(f"{name} must not be an expanded view")
-
-
-def _ints(name, x, shape, device):
-    import torch
-    if x.dtype != torch.int32 or tuple(x.shape) != tuple(shape) or not x.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}, got {x.dtype} {tuple(x.shape)}")
-    _on(name, x, device)
-    return x.data_ptr()
+        import torch  # noqa: F401  (its libraries are loaded first)
+        N.lib()
+        if not N.BIND_PATH.exists():
+            raise N.NativeLibraryMissing(f"{N.BIND_PATH} is not built; run `python -m ffn_residual_mesh_b200.build`")
+        spec = importlib.util.spec_from_file_location("ffnrm_kv_bind", N.BIND_PATH)
+        _module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_module)
+    return _module
 
 
 class RotaryTable:
@@ -132,26 +115,7 @@ def rotary(x, positions, table: RotaryTable, out=None, inverse: bool = False, st
     """x [T, heads, dim] with its first ``rotary_dim`` channels rotated at ``positions`` (int32
     [T]); ``inverse`` applies the transposed rotation, the gradient of the forward one.
     ``out`` may be x. A position outside the table gives NaN in the rotated channels."""
-    import torch
-    if x.dim() != 3:
-        raise ValueError(f"x must have shape (T, heads, dim), got {tuple(x.shape)}")
-    T, heads, dim = x.shape
-    if table.rotary_dim > dim:
-        raise ValueError(f"rotary_dim={table.rotary_dim} exceeds head dim {dim}")
-    if out is None:
-        out = torch.empty((T, heads, dim), dtype=x.dtype, device=x.device)
-    if out.dtype != x.dtype or out.shape != x.shape:
-        raise ValueError("out must have x's type and shape")
-    _writable("out", out)
-    for name, t in (("out", out), ("table", table.cos_sin)):
-        _on(name, t, x.device)
-    dtype, xr, yr = _dtype(x), _rows("x", x, heads, dim), _rows("out", out, heads, dim)
-    pos = _ints("positions", positions, (T,), x.device)
-    with torch.cuda.device(x.device):
-        N.check(N.lib().ffnrm_rotary(ctypes.byref(xr), ctypes.byref(yr), dtype, T, heads, dim, pos,
-                                     table.cos_sin.data_ptr(), table.rotary_dim, table.max_positions,
-                                     table.flags | (N.ROTARY_INVERSE if inverse else 0), _stream(stream)))
-    return out
+    return (_module or _bind()).rotary(x, positions, table.cos_sin, out, table.flags | (N.ROTARY_INVERSE if inverse else 0), stream)
 
 
 class PagedKvCache:
@@ -166,6 +130,7 @@ class PagedKvCache:
         import torch
         self.handle = None
         self.lib = N.lib()
+        self._calls = _bind()
         self.n_layers, self.n_pages, self.kv_heads, self.head_dim = n_layers, n_pages, kv_heads, head_dim
         self.page_tokens, self.max_seqs = page_tokens, max_seqs
         self.device = torch.device("cuda", device)
@@ -182,17 +147,20 @@ class PagedKvCache:
             if tuple(b.shape) != shape or b.dtype != dtype or not b.is_contiguous():
                 raise ValueError(f"a cache buffer must be a contiguous {dtype} tensor of shape {shape}, "
                                  f"got {b.dtype} {tuple(b.shape)}")
-            _on("a cache buffer", b, self.device)
+            if b.device != self.device:
+                raise ValueError(f"a cache buffer must be on {self.device}, got {b.device}")
         self.k_codes, self.v_codes, self.k_scale, self.v_scale = buffers
         cfg = N.KvConfig(n_layers, n_pages, kv_heads, head_dim, page_tokens, max_seqs)
         handle = ctypes.c_void_p()
         N.check(self.lib.ffnrm_kv_create(ctypes.byref(handle), device, ctypes.byref(cfg),
                                          *(b.data_ptr() for b in buffers)))
         self.handle = handle
+        self._geo = (handle.value, kv_heads, head_dim, device)
 
     # -- lifetime ---------------------------------------------------------
     def close(self) -> None:
         if getattr(self, "handle", None):
+            self._geo = None
             N.check(self.lib.ffnrm_kv_destroy(self.handle))
             self.handle = None
 
@@ -211,19 +179,8 @@ class PagedKvCache:
     def check(self, stream=None) -> None:
         """Synchronise and raise what the kernels recorded: MemoryError (too few free pages),
         TimeoutError (a bounded wait ran out), RuntimeError (data that could not be used)."""
-        N.check(self.lib.ffnrm_kv_check(self.handle, self._stream(stream)))
-
-    def _stream(self, stream):
         import torch
-        return _stream(torch.cuda.current_stream(self.device) if stream is None else stream)
-
-    def _batch(self, tables, lengths, starts, rows) -> N.KvBatch:
-        if tables.dim() != 2:
-            raise ValueError(f"tables must have shape (seqs, width), got {tuple(tables.shape)}")
-        seqs, width = tables.shape
-        return N.KvBatch(_ints("tables", tables, (seqs, width), self.device),
-                         _ints("lengths", lengths, (seqs,), self.device),
-                         None if starts is None else _ints("starts", starts, (seqs + 1,), self.device), seqs, width, rows)
+        N.check(self.lib.ffnrm_kv_check(self.handle, _stream(torch.cuda.current_stream(self.device) if stream is None else stream)))
 
     # -- a step's work --------------------------------------------------------
     def append(self, layer: int, k, v, tables, lengths, starts=None, rope: RotaryTable | None = None, q=None, q_out=None,
@@ -231,38 +188,8 @@ class PagedKvCache:
         """Quantise the step's new k and v [T, kv_heads, head_dim] into their pages. With
         ``rope`` the keys are rotated at their positions first, and with ``q`` [T, heads,
         head_dim] the queries too; returns the rotated queries (``q_out``, which may be q)."""
-        import torch
-        T = k.shape[0] if k.dim() == 3 else -1
-        kr, vr = _rows("k", k, self.kv_heads, self.head_dim), _rows("v", v, self.kv_heads, self.head_dim, T)
-        dtype = _dtype(k)
-        if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
-            raise ValueError("q, k and v must have one type")
-        batch = self._batch(tables, lengths, starts, T)
-        for name, t in (("k", k), ("v", v)):
-            _on(name, t, self.device)
-        qr = yr = None
-        q_heads = 0
-        if q is not None:
-            if rope is None:
-                raise ValueError("q is only rotated: it needs rope")
-            q_heads = q.shape[1] if q.dim() == 3 else -1
-            qr = _rows("q", q, q_heads, self.head_dim, T)
-            _on("q", q, self.device)
-            if q_out is None:
-                q_out = torch.empty((T, q_heads, self.head_dim), dtype=q.dtype, device=self.device)
-            yr = _rows("q_out", q_out, q_heads, self.head_dim, T)
-            _on("q_out", q_out, self.device)
-            _writable("q_out", q_out)
-            if q_out.dtype != q.dtype:
-                raise ValueError("q_out must have q's type")
-        if rope is not None:
-            _on("rope", rope.cos_sin, self.device)
-        N.check(self.lib.ffnrm_kv_append(
-            self.handle, layer, ctypes.byref(batch), dtype, ctypes.byref(kr), ctypes.byref(vr),
-            ctypes.byref(qr) if qr else None, ctypes.byref(yr) if yr else None, q_heads,
-            rope.cos_sin.data_ptr() if rope else None, rope.rotary_dim if rope else 0, rope.max_positions if rope else 0,
-            rope.flags if rope else 0, self._stream(stream)))
-        return q_out
+        return self._calls.append(self._geo, layer, k, v, tables, lengths, starts, rope.cos_sin if rope else None,
+                                  rope.flags if rope else 0, q, q_out, stream)
 
     def attend(self, layer: int, q, tables, lengths, starts=None, out=None, lse=None, scale: float | None = None,
                causal: bool = True, window: int = 0, stream=None):
@@ -270,40 +197,17 @@ class PagedKvCache:
         cache, the step's own tokens included. ``scale`` defaults to ``head_dim ** -0.5``;
         ``window`` > 0 lets a query see its last ``window`` positions only. ``lse`` (float32
         [T, heads]) receives the natural log of the sum of exponentials."""
-        import torch
-        if q.dim() != 3 or q.shape[1] % self.kv_heads or q.shape[1] == 0:
-            raise ValueError(f"q must have shape (T, a multiple of {self.kv_heads}, {self.head_dim}), got {tuple(q.shape)}")
-        T, heads = q.shape[:2]
-        dtype, qr = _dtype(q), _rows("q", q, heads, self.head_dim)
-        batch = self._batch(tables, lengths, starts, T)
-        if out is None:
-            out = torch.empty((T, heads, self.head_dim), dtype=q.dtype, device=self.device)
-        yr = _rows("out", out, heads, self.head_dim, T)
-        for name, t in (("q", q), ("out", out)):
-            _on(name, t, self.device)
-        _writable("out", out)
-        if out.dtype != q.dtype:
-            raise ValueError("out must have q's type")
-        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (T, heads) or not lse.is_contiguous()):
-            raise ValueError(f"lse must be a contiguous float32 tensor of shape ({T}, {heads})")
-        if lse is not None:
-            _on("lse", lse, self.device)
-        N.check(self.lib.ffnrm_kv_attend(
-            self.handle, layer, ctypes.byref(batch), dtype, ctypes.byref(qr), ctypes.byref(yr),
-            None if lse is None else lse.data_ptr(), heads, self.head_dim ** -0.5 if scale is None else float(scale),
-            int(bool(causal)), int(window), self._stream(stream)))
-        return out
+        return self._calls.attend(self._geo, layer, q, tables, lengths, starts, out, lse,
+                                  self.head_dim ** -0.5 if scale is None else scale, causal, window, stream)
 
     def read(self, layer: int, tables, lengths, starts, rows: int, dtype=None, stream=None):
         """The last tokens of each sequence back from the cache: k and v [rows, kv_heads,
         head_dim] (code * scale), float32 unless ``dtype``. ``starts`` says how many of each."""
         import torch
-        dtype = torch.float32 if dtype is None else dtype
-        batch = self._batch(tables, lengths, starts, rows)
-        k, v = (torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
-        N.check(self.lib.ffnrm_kv_read(self.handle, layer, ctypes.byref(batch), _dtype(k), k.data_ptr(), v.data_ptr(),
-                                       self._stream(stream)))
-        return k, v
+        types = {None: N.F32, torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
+        if dtype not in types:
+            raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+        return self._calls.read(self._geo, layer, tables, lengths, starts, rows, types[dtype], stream)
 
     # -- pages between steps --------------------------------------------------
     def fork(self, tables, lengths, parents, extra, out_tables=None, out_lengths=None, info=None, stream=None):
@@ -311,47 +215,15 @@ class PagedKvCache:
         with room for ``extra[i]`` new tokens. A sequence named by several children is
         shared (its open last page is copied), one named by none is freed. Returns (tables,
         lengths, info); info int32 [4] holds the pages held, free, copied and short."""
-        import torch
-        if tables.dim() != 2 or parents.dim() != 1:
-            raise ValueError("tables must have shape (seqs, width), parents (children,)")
-        seqs, width = tables.shape
-        n = parents.shape[0]
-        if out_tables is None:
-            out_tables = torch.empty((n, width), dtype=torch.int32, device=self.device)
-        if out_lengths is None:
-            out_lengths = torch.empty((n,), dtype=torch.int32, device=self.device)
-        if info is None:
-            info = torch.empty((4,), dtype=torch.int32, device=self.device)
-        if out_tables.dim() != 2:
-            raise ValueError("out_tables must have shape (children, width)")
-        d = self.device
-        N.check(self.lib.ffnrm_kv_fork(
-            self.handle, _ints("tables", tables, (seqs, width), d), _ints("lengths", lengths, (seqs,), d), seqs, width,
-            _ints("parents", parents, (n,), d), _ints("extra", extra, (n,), d), n,
-            _ints("out_tables", out_tables, (n, out_tables.shape[1]), d), out_tables.shape[1],
-            _ints("out_lengths", out_lengths, (n,), d), _ints("info", info, (4,), d), self._stream(stream)))
-        return out_tables, out_lengths, info
+        return self._calls.fork(self._geo, tables, lengths, parents, extra, out_tables, out_lengths, info, stream)
 
     def compact(self, tables, lengths, out_tables=None, info=None, stream=None):
         """Move the held pages to the lowest ids. Returns (tables, info); ``out_tables`` may be
         ``tables``. No held page is overwritten, so the old tables stay readable until the
         next fork hands out the freed pages."""
-        import torch
-        if tables.dim() != 2:
-            raise ValueError("tables must have shape (seqs, width)")
-        seqs, width = tables.shape
-        if out_tables is None:
-            out_tables = torch.empty_like(tables)
-        if info is None:
-            info = torch.empty((4,), dtype=torch.int32, device=self.device)
-        d = self.device
-        N.check(self.lib.ffnrm_kv_compact(
-            self.handle, _ints("tables", tables, (seqs, width), d), _ints("lengths", lengths, (seqs,), d), seqs, width,
-            _ints("out_tables", out_tables, (seqs, width), d), _ints("info", info, (4,), d), self._stream(stream)))
-        return out_tables, info
+        return self._calls.compact(self._geo, tables, lengths, out_tables, info, stream)
 
     def copy_pages(self, src, dst, stream=None) -> None:
-        """Copy page src[i] to dst[i] in every layer (int32 [n]; no page is named twice)."""
-        n = src.shape[0] if src.dim() == 1 else -1
-        N.check(self.lib.ffnrm_kv_copy_pages(self.handle, _ints("src", src, (n,), self.device),
-                                             _ints("dst", dst, (n,), self.device), n, self._stream(stream)))
+        """Copy page src[i] to dst[i] in every layer (int32 [n]; a destination is named once and is
+        no source)."""
+        self._calls.copy_pages(self._geo, src, dst, stream)
