@@ -6,7 +6,9 @@
 // to the operand registers: a thread reads 16 contiguous channels of a key (and of four keys of V),
 // and since the contracted index may be permuted as long as both operands agree, the bytes are
 // in place as they come. int8 -> f16 is exact: byte ^ 0x80 under the exponent of 1024 gives
-// 1152 + q, minus 1152. S^T becomes P^T's operand by one 8x8 transpose per 8 keys.
+// 1152 + q, minus 1152 (leaving the bias in K's operand and starting S from -1152 sum q would save 32 of
+// some 400 instructions per tile, but cost a logit 2e-5). S^T becomes P^T's operand by one 8x8
+// transpose per 8 keys.
 //
 // The running maximum moves only when a score passes it by 2^8 (p stays below 2^15 in f16 with
 // the 2^7 offset), which a vote per 16 keys decides.
@@ -76,9 +78,13 @@ struct FewArgs {
     int most_rows;   // sequences with more rows belong to the other kernel
 };
 
-// The stretch of a sequence that its rows see, in units of UK keys, and its row tiles.
+// The stretch of a sequence that its rows see, in units of UK keys, and its row tiles. On the line an item
+// takes kFewItem units more, about what its queries, first loads and output cost beside the keys
+// (without them a block with 18 short items ran three times as long as one with 50 units of one).
+constexpr int kFewItem = 3;
 struct SeqWork {
     int first, n, length, unit0, units, tiles;
+    __device__ __forceinline__ int span() const { return units ? units + kFewItem : 0; }
 };
 template <int UK, int RT>
 __device__ __forceinline__ SeqWork seq_work(const AttendArgs &a, int s, int most_rows) {
@@ -99,11 +105,14 @@ __device__ __forceinline__ SeqWork seq_work(const AttendArgs &a, int s, int most
 // Bytes of dynamic shared memory and floats of one partial.
 template <int D, int NT, int W>
 constexpr int few_smem() { return W * 8 * NT * (D + 2) * 4; }
+// Blocks that an SM should hold: the keys under way are what the registers of its warps hold.
+template <int D, int NT>
+constexpr int few_blocks() { return D == 64 ? (NT == 1 ? 5 : 3) : D == 128 ? (NT == 1 ? 4 : 2) : 2; }
 template <int D, int NT>
 constexpr int few_slot() { return 8 * NT * (D + 2); }
 
 template <typename T, int D, int NT, int W>
-__global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
+__global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel(FewArgs f) {
     constexpr float kLog2e = 1.4426950408889634f;
     constexpr int RT = 8 * NT, UK = 16 * W, KV = D / 64, MT = D / 16, VB = D / 8;
     const AttendArgs &a = f.a;
@@ -121,7 +130,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
         int64_t u = 0;
         if (s0 + lane < a.batch.seqs) {
             const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
-            u = int64_t(w.units) * w.tiles * pl.heads;
+            u = int64_t(w.span()) * w.tiles * pl.heads;
         }
         for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
         total += u;
@@ -137,7 +146,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
         int64_t u = 0;
         if (s0 + lane < a.batch.seqs) {
             const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
-            u = int64_t(w.units) * w.tiles * pl.heads;
+            u = int64_t(w.span()) * w.tiles * pl.heads;
         }
         int64_t run = u;
         for (int o = 1; o < 32; o <<= 1) {
@@ -156,15 +165,19 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
 
     while (at < end && s < a.batch.seqs) {
         const SeqWork w = seq_work<UK, RT>(a, s, f.most_rows);
-        const int64_t item = w.units ? (at - seq_at) / w.units : 0;
+        const int64_t item = w.units ? (at - seq_at) / w.span() : 0;
         if (w.units == 0 || item >= int64_t(w.tiles) * pl.heads) {
-            seq_at += int64_t(w.units) * w.tiles * pl.heads;
+            seq_at += int64_t(w.span()) * w.tiles * pl.heads;
             ++s;
             continue;
         }
         const int tile = int(item % w.tiles), h = int(item / w.tiles);
-        const int64_t item_at = seq_at + item * w.units;
-        const int u0 = int(at - item_at), u1 = int(min(int64_t(w.units), end - item_at));
+        const int64_t item_at = seq_at + item * w.span(), item_end = item_at + w.span();
+        const int u0 = max(0, int(at - item_at) - kFewItem), u1 = int(min(item_end, end) - item_at) - kFewItem;
+        if (u1 <= u0) {  // the block's stretch ends before the item's first key
+            at = min(item_end, end);
+            continue;
+        }
         const int rows = min(RT, w.n * a.group - tile * RT), pos0 = w.length - w.n;
         const int32_t *table = a.batch.tables + int64_t(s) * a.batch.width;
 
@@ -233,78 +246,70 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
             for (int i = 0; i < MT; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
         }
 
-        uint4 kr[2 * KV];
-        uint2 vr[4 * (VB / 8)];
-        float sk = 0.f, sv = 1.f;
-        bool have = false;
+        // A tile of 16 keys in registers: K words of keys g and g + 8, V words of keys 2t, 2t + 1, 2t + 8,
+        // 2t + 9. Each half is loaded again as soon as its product has used it.
+        uint32_t xk[KV][2][4], xv[4][VB / 4];
+        float ks = 0.f, vs = 1.f;
         auto key_of = [&](int u) { return (w.unit0 + u) * UK + warp * 16; };
         auto page_of = [&](int u) {
             const int key = key_of(u);
             return u < u1 && key < any_hi && key + 16 > any_lo ? table[key >> pl.page_shift] : -2;
         };
-        auto load = [&](int u, int page) {
-            have = page >= 0 && page < pl.pages;
-            if (!have) {
-                if (page != -2 && lane == 0) atomicOr(a.status, kStatusPage);
-                return;
-            }
-            const int off = key_of(u) & (pl.page_tokens - 1);
-            const int64_t ph = int64_t(page) * pl.heads + h;
-            const int64_t base = (ph * pl.page_tokens + off) * D;
-            const int8_t *kp = pl.k_codes + base + g * D + t * 16, *vp = pl.v_codes + base + (2 * t) * D + g * (VB < 16 ? VB : 16);
-#pragma unroll
-            for (int j = 0; j < KV; ++j) {
-                kr[2 * j] = ldg_stream16(kp + j * 64);
-                kr[2 * j + 1] = ldg_stream16(kp + 8 * D + j * 64);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int8_t *p = vp + (r & 1) * D + (r >> 1) * 8 * D;
-                if constexpr (VB == 8) {
-                    vr[r] = ldg_stream8(p);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VB / 16; ++j) {
-                        const uint4 x = ldg_stream16(p + j * 128);
-                        vr[r * (VB / 8) + 2 * j] = make_uint2(x.x, x.y);
-                        vr[r * (VB / 8) + 2 * j + 1] = make_uint2(x.z, x.w);
-                    }
-                }
-            }
-            sk = pl.k_scale[ph];
-            sv = pl.v_scale[ph];
+        auto valid = [&](int page) {
+            const bool have = unsigned(page) < unsigned(pl.pages);
+            if (!have && page != -2 && lane == 0) atomicOr(a.status, kStatusPage);
+            return have;
         };
-
-        load(u0, page_of(u0));
-        int next_page = page_of(u0 + 1);
-        for (int u = u0; u < u1; ++u) {
-            const int key = key_of(u);
-            const bool now = have;
-            uint32_t ka[KV][2][4], va[4][VB / 4];
+        auto load_k = [&](int u, int page) {
+            const int64_t ph = int64_t(page) * pl.heads + h;
+            const int8_t *kp = pl.k_codes + (ph * pl.page_tokens + (key_of(u) & (pl.page_tokens - 1))) * D + g * D + t * 16;
 #pragma unroll
             for (int j = 0; j < KV; ++j)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    ka[j][i][0] = kr[2 * j + i].x;
-                    ka[j][i][1] = kr[2 * j + i].y;
-                    ka[j][i][2] = kr[2 * j + i].z;
-                    ka[j][i][3] = kr[2 * j + i].w;
+                    const uint4 y = ldg_stream16(kp + i * 8 * D + j * 64);
+                    xk[j][i][0] = y.x, xk[j][i][1] = y.y, xk[j][i][2] = y.z, xk[j][i][3] = y.w;
                 }
+        };
+        auto load_v = [&](int u, int page) {
+            const int64_t ph = int64_t(page) * pl.heads + h;
+            const int8_t *vp = pl.v_codes + (ph * pl.page_tokens + (key_of(u) & (pl.page_tokens - 1))) * D + (2 * t) * D + g * (VB < 16 ? VB : 16);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r) {
+                const int8_t *p = vp + (r & 1) * D + (r >> 1) * 8 * D;
+                if constexpr (VB == 8) {
+                    const uint2 y = ldg_stream8(p);
+                    xv[r][0] = y.x, xv[r][1] = y.y;
+                } else {
 #pragma unroll
-                for (int j = 0; j < VB / 8; ++j) {
-                    va[r][2 * j] = vr[r * (VB / 8) + j].x;
-                    va[r][2 * j + 1] = vr[r * (VB / 8) + j].y;
+                    for (int j = 0; j < VB / 16; ++j) {
+                        const uint4 y = ldg_stream16(p + j * 128);
+                        xv[r][4 * j] = y.x, xv[r][4 * j + 1] = y.y, xv[r][4 * j + 2] = y.z, xv[r][4 * j + 3] = y.w;
+                    }
                 }
-            // a NaN value scale reaches the rows that see it through vlog; it must not meet the others' p = 0
-            const float ks = sk, vlog = lg2(sv), vinv = sv == sv ? __fdividef(1.f, sv) : 0.f;
-            if (u + 1 < u1) {
-                load(u + 1, next_page);
-                next_page = page_of(u + 2);
             }
-            if (!now) continue;
-
+            ks = pl.k_scale[ph];
+            vs = pl.v_scale[ph];
+        };
+        int page = page_of(u0), next_page = page_of(u0 + 1);
+        bool have = valid(page);
+        if (have) {
+            load_k(u0, page);
+            load_v(u0, page);
+        }
+        for (int u = u0; u < u1; ++u) {
+            const bool next = valid(next_page);
+            const int key = key_of(u), this_page = next_page;
+            next_page = page_of(u + 2);
+            if (!have) {
+                have = next;
+                if (next) {
+                    load_k(u + 1, this_page);
+                    load_v(u + 1, this_page);
+                }
+                continue;
+            }
+            have = next;
             // S^T = K Q^T: 16 keys x 8 NT rows
             float sc[NT][4];
 #pragma unroll
@@ -313,12 +318,15 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
             for (int j = 0; j < KV; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const uint32_t x = ka[j][0][k] ^ 0x80808080u, y = ka[j][1][k] ^ 0x80808080u;
-                    const uint32_t a0 = codes_f16x2<0>(x), a1 = codes_f16x2<0>(y), a2 = codes_f16x2<1>(x), a3 = codes_f16x2<1>(y);
+                    const uint32_t y = xk[j][0][k] ^ 0x80808080u, z = xk[j][1][k] ^ 0x80808080u;
+                    const uint32_t a0 = codes_f16x2<0>(y), a1 = codes_f16x2<0>(z), a2 = codes_f16x2<1>(y), a3 = codes_f16x2<1>(z);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma16816(sc[n], a0, a1, a2, a3, qb[n][j * 4 + k][0], qb[n][j * 4 + k][1]);
                 }
-            // z = y log2(e) + log2(sv); sc[n][i + 2 k]: key + g + 8 k, row 2t + i
+            if (next) load_k(u + 1, this_page);
+            // z = y log2(e) + log2(sv); sc[n][i + 2 k]: key + g + 8 k, row 2t + i. A NaN value scale reaches the
+            // rows that see it through its logarithm; it must not meet the others' p = 0.
+            const float vlog = lg2(vs), vinv = vs == vs ? __fdividef(1.f, vs) : 0.f;
             const bool whole = key + 16 <= all_hi && key >= all_lo;
             bool raise = false;
 #pragma unroll
@@ -327,17 +335,22 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
                 for (int i = 0; i < 2; ++i) {
                     const float f0 = qs[n][i] * ks;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        float z = fmaf(sc[n][i + 2 * k], f0, vlog);
-                        if (!whole) {
-                            const int j = key + g + 8 * k;
-                            const bool seen = j < w.length && (!a.causal || j <= qp[n][i]) && (a.window <= 0 || j > qp[n][i] - a.window);
-                            z = seen ? z : ninf;
-                        }
-                        raise |= z > m[n][i] + kFewStep;
-                        sc[n][i + 2 * k] = z;
-                    }
+                    for (int k = 0; k < 2; ++k) sc[n][i + 2 * k] = fmaf(sc[n][i + 2 * k], f0, vlog);
                 }
+            if (!whole) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = key + g + 8 * (i >> 1), p = qp[n][i & 1];
+                        const bool seen = j < w.length && (!a.causal || j <= p) && (a.window <= 0 || j > p - a.window);
+                        sc[n][i] = seen ? sc[n][i] : ninf;
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) raise |= fmaxf(sc[n][i], sc[n][i + 2]) > m[n][i] + kFewStep;
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -352,9 +365,9 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
                         m[n][i] = top;
                         l[n][i] *= fix;
 #pragma unroll
-                        for (int x = 0; x < MT; ++x) {
-                            o[x][n][i] *= fix;
-                            o[x][n][i + 2] *= fix;
+                        for (int c = 0; c < MT; ++c) {
+                            o[c][n][i] *= fix;
+                            o[c][n][i + 2] *= fix;
                         }
                     }
             }
@@ -374,17 +387,18 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
             }
             // O^T += V^T P^T: channels (thread g: 16 g + ..) x rows, over the 16 keys
 #pragma unroll
-            for (int x = 0; x < VB / 4; ++x) {  // 4 channels each
-                const uint32_t lo01 = __byte_perm(va[0][x], va[1][x], 0x5140) ^ 0x80808080u, lo23 = __byte_perm(va[0][x], va[1][x], 0x7362) ^ 0x80808080u;
-                const uint32_t hi01 = __byte_perm(va[2][x], va[3][x], 0x5140) ^ 0x80808080u, hi23 = __byte_perm(va[2][x], va[3][x], 0x7362) ^ 0x80808080u;
+            for (int c = 0; c < VB / 4; ++c) {  // 4 channels each
+                const uint32_t lo01 = __byte_perm(xv[0][c], xv[1][c], 0x5140) ^ 0x80808080u, lo23 = __byte_perm(xv[0][c], xv[1][c], 0x7362) ^ 0x80808080u;
+                const uint32_t hi01 = __byte_perm(xv[2][c], xv[3][c], 0x5140) ^ 0x80808080u, hi23 = __byte_perm(xv[2][c], xv[3][c], 0x7362) ^ 0x80808080u;
                 const uint32_t a0 = codes_f16x2<0>(lo01), a1 = codes_f16x2<1>(lo01), a2 = codes_f16x2<0>(hi01), a3 = codes_f16x2<1>(hi01);
                 const uint32_t b0 = codes_f16x2<0>(lo23), b1 = codes_f16x2<1>(lo23), b2 = codes_f16x2<0>(hi23), b3 = codes_f16x2<1>(hi23);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma16816(o[2 * x][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-                    mma16816(o[2 * x + 1][n], b0, b1, b2, b3, pb[n][0], pb[n][1]);
+                    mma16816(o[2 * c][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+                    mma16816(o[2 * c + 1][n], b0, b1, b2, b3, pb[n][0], pb[n][1]);
                 }
             }
+            if (next) load_v(u + 1, this_page);
         }
 
         // Join the warps. Row r's sums over the keys are spread over g.
@@ -454,8 +468,8 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
         }
         if (split) {
             // blocks that hold a piece of this item: unit u lies in block floor(((u + 1) blocks - 1) / total)
-            const int b0 = int(((item_at + 1) * blocks - 1) / total);
-            const int b1 = int(((item_at + w.units) * blocks - 1) / total);
+            const int b0 = int(((item_at + kFewItem + 1) * blocks - 1) / total);
+            const int b1 = int((item_end * blocks - 1) / total);
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -498,7 +512,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(FewArgs f) {
                 }
             }
         }
-        at = item_at + u1;
+        at = min(item_end, end);
     }
 }
 
