@@ -150,7 +150,7 @@ void launch_append(const AppendArgs &a, bool vec, bool interleaved, unsigned gri
         append_kernel<T, false, false><<<grid, 256, 0, st>>>(a);
 }
 
-constexpr int kFewWarps = 4, kFewMinUnits = 2;
+constexpr int kFewWarps = 8, kFewMinUnits = 1;
 // Sequences with more query rows (tokens x group) than this take the tcgen05 kernel.
 constexpr int kFewRows = 64;
 

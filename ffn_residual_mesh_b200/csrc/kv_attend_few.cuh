@@ -70,6 +70,14 @@ __device__ __forceinline__ uint2 ldg_stream8(const int8_t *p) {
     return v;
 }
 
+// floor(a b / n) for the split of the line, in 32 bits where they are enough (a 64-bit division takes a
+// tenth of a microsecond at the start of every block).
+__device__ __forceinline__ int64_t share(int64_t a, int64_t b, int64_t n) {
+    const uint64_t x = uint64_t(a) * uint64_t(b);
+    if ((x | uint64_t(n)) >> 32 == 0) return uint32_t(x) / uint32_t(n);
+    return int64_t(x / uint64_t(n));
+}
+
 struct FewArgs {
     AttendArgs a;
     float *partial;  // [2 * gridDim.x][rows of a tile][D + 2]
@@ -105,14 +113,63 @@ __device__ __forceinline__ SeqWork seq_work(const AttendArgs &a, int s, int most
 // Bytes of dynamic shared memory and floats of one partial.
 template <int D, int NT, int W>
 constexpr int few_smem() { return W * 8 * NT * (D + 2) * 4; }
-// Blocks that an SM should hold: the keys under way are what the registers of its warps hold.
+// Blocks of W warps that an SM should hold: the keys under way are what the registers of its warps hold.
+template <int D, int NT, int W>
+constexpr int few_blocks() { return (D == 64 ? (NT == 1 ? 20 : 12) : D == 128 ? (NT == 1 ? 16 : 8) : 8) / W; }
 template <int D, int NT>
-constexpr int few_blocks() { return D == 64 ? (NT == 1 ? 5 : 3) : D == 128 ? (NT == 1 ? 4 : 2) : 2; }
-template <int D, int NT>
-constexpr int few_slot() { return 8 * NT * (D + 2); }
+__host__ __device__ constexpr int few_slot() { return 8 * NT * (D + 2); }
+
+// The item's rows from the pieces that blocks b0 .. b1 left, in their order. (A call of its own, so that
+// the loads under way here take no registers from the loop over the keys.)
+template <typename T, int D, int NT, int W>
+__device__ __noinline__ void join_pieces(const FewArgs &f, int b0, int b1, bool second, int h, int tile, int rows, int first) {
+    constexpr int RT = 8 * NT, SLOT = few_slot<D, NT>(), GO = 8;  // pieces under way at a time
+    const AttendArgs &a = f.a;
+    const float ninf = -__int_as_float(0x7f800000);
+    for (int e = threadIdx.x; e < rows * (D / 4); e += W * 32) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4;
+        float top = ninf, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int b = b0; b <= b1; b += GO) {
+            float mk[GO], lk[GO];
+            float4 x[GO];
+#pragma unroll
+            for (int i = 0; i < GO; ++i) {
+                // block b0 may have worked on another item before; every other one begins with this one
+                const int at = min(b + i, b1);
+                const float *p = f.partial + int64_t(2 * at + (at == b0 && second ? 1 : 0)) * SLOT;
+                mk[i] = __ldcg(p + RT * D + r);
+                lk[i] = __ldcg(p + RT * D + RT + r);
+                x[i] = __ldcg(reinterpret_cast<const float4 *>(p + r * D + d));
+            }
+#pragma unroll
+            for (int i = 0; i < GO; ++i) {
+                if (b + i > b1) break;
+                const float to = fmaxf(top, mk[i]);
+                const float fa = top == ninf ? (sum != sum ? 1.f : 0.f) : ex2(top - to);
+                const float fb = mk[i] == ninf ? (lk[i] != lk[i] ? 1.f : 0.f) : ex2(mk[i] - to);
+                acc.x = acc.x * fa + x[i].x * fb;
+                acc.y = acc.y * fa + x[i].y * fb;
+                acc.z = acc.z * fa + x[i].z * fb;
+                acc.w = acc.w * fa + x[i].w * fb;
+                sum = sum * fa + lk[i] * fb;
+                top = to;
+            }
+        }
+        const int q = tile * RT + r, token = q / a.group, hq = h * a.group + q - token * a.group;
+        const float norm = sum == 0.f ? 0.f : 1.f / sum;
+        Vec<T, 4> y;
+        y.v[0] = from_f32<T>(acc.x * norm), y.v[1] = from_f32<T>(acc.y * norm);
+        y.v[2] = from_f32<T>(acc.z * norm), y.v[3] = from_f32<T>(acc.w * norm);
+        *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (first + token) * a.o_token + hq * a.o_head + d) = y;
+        if (a.lse && d == 0)
+            a.lse[int64_t(first + token) * (a.pool.heads * a.group) + hq] =
+                sum == 0.f ? ninf : (top - kFewOffset + lg2(sum)) * 0.6931471805599453f;
+    }
+}
 
 template <typename T, int D, int NT, int W>
-__global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel(FewArgs f) {
+__global__ void __launch_bounds__(W * 32, few_blocks<D, NT, W>()) attend_few_kernel(const __grid_constant__ FewArgs f) {
     constexpr float kLog2e = 1.4426950408889634f;
     constexpr int RT = 8 * NT, UK = 16 * W, KV = D / 64, MT = D / 16, VB = D / 8;
     const AttendArgs &a = f.a;
@@ -125,28 +182,32 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel
 
     zero_loose_rows<T>(a);
     // This block's stretch of the line of units.
-    int64_t total = 0;
+    int64_t total = 0, mine = 0;
     for (int s0 = 0; s0 < a.batch.seqs; s0 += 32) {
         int64_t u = 0;
         if (s0 + lane < a.batch.seqs) {
             const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
             u = int64_t(w.span()) * w.tiles * pl.heads;
         }
+        mine = u;
         for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
         total += u;
     }
     if (total == 0) return;
-    const int64_t blocks = min(int64_t(gridDim.x), (total + f.min_units - 1) / f.min_units);
+    const int64_t blocks = min(int64_t(gridDim.x), share(total + f.min_units - 1, 1, f.min_units));
     if (blockIdx.x >= blocks) return;
-    int64_t at = total * blockIdx.x / blocks;
-    const int64_t end = total * (blockIdx.x + 1) / blocks, start = at;
+    int64_t at = share(total, blockIdx.x, blocks);
+    const int64_t end = share(total, blockIdx.x + 1, blocks), start = at;
     int s = 0;
     int64_t seq_at = 0;  // line position of sequence s
     for (int s0 = 0; s0 < a.batch.seqs; s0 += 32) {
-        int64_t u = 0;
-        if (s0 + lane < a.batch.seqs) {
-            const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
-            u = int64_t(w.span()) * w.tiles * pl.heads;
+        int64_t u = mine;
+        if (a.batch.seqs > 32) {
+            u = 0;
+            if (s0 + lane < a.batch.seqs) {
+                const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
+                u = int64_t(w.span()) * w.tiles * pl.heads;
+            }
         }
         int64_t run = u;
         for (int o = 1; o < 32; o <<= 1) {
@@ -165,13 +226,13 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel
 
     while (at < end && s < a.batch.seqs) {
         const SeqWork w = seq_work<UK, RT>(a, s, f.most_rows);
-        const int64_t item = w.units ? (at - seq_at) / w.span() : 0;
+        const int64_t item = w.units ? share(at - seq_at, 1, w.span()) : 0;
         if (w.units == 0 || item >= int64_t(w.tiles) * pl.heads) {
             seq_at += int64_t(w.span()) * w.tiles * pl.heads;
             ++s;
             continue;
         }
-        const int tile = int(item % w.tiles), h = int(item / w.tiles);
+        const int h = int(share(item, 1, w.tiles)), tile = int(item - int64_t(h) * w.tiles);
         const int64_t item_at = seq_at + item * w.span(), item_end = item_at + w.span();
         const int u0 = max(0, int(at - item_at) - kFewItem), u1 = int(min(item_end, end) - item_at) - kFewItem;
         if (u1 <= u0) {  // the block's stretch ends before the item's first key
@@ -181,11 +242,25 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel
         const int rows = min(RT, w.n * a.group - tile * RT), pos0 = w.length - w.n;
         const int32_t *table = a.batch.tables + int64_t(s) * a.batch.width;
 
+        const int token_lo = tile * RT / a.group, token_hi = (tile * RT + rows - 1) / a.group;
+        // keys that every row of the tile sees: [all_lo, all_hi); that any sees: [any_lo, any_hi)
+        const int any_hi = a.causal ? min(w.length, pos0 + token_hi + 1) : w.length;
+        const int all_hi = a.causal ? min(w.length, pos0 + token_lo + 1) : w.length;
+        const int any_lo = a.window > 0 ? max(0, pos0 + token_lo - a.window + 1) : 0;
+        const int all_lo = a.window > 0 ? max(0, pos0 + token_hi - a.window + 1) : 0;
+
+        auto key_of = [&](int u) { return (w.unit0 + u) * UK + warp * 16; };
+        auto page_of = [&](int u) {
+            const int key = key_of(u);
+            return u < u1 && key < any_hi && key + 16 > any_lo ? table[key >> pl.page_shift] : -2;
+        };
+        const int page = page_of(u0);
+        int next_page = page_of(u0 + 1);  // on their way while the queries are read
+
         // queries: B operands, and per row the position and the scale
         uint32_t qb[NT][D / 16][2];
         float qs[NT][2];
         int qp[NT][2];
-        const int token_lo = tile * RT / a.group, token_hi = (tile * RT + rows - 1) / a.group;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int r = tile * RT + n * 8 + g;
@@ -231,12 +306,6 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel
                 qp[n][i] = __shfl_sync(0xffffffffu, ps, (2 * t + i) * 4);
             }
         }
-        // keys that every row of the tile sees: [all_lo, all_hi); that any sees: [any_lo, any_hi)
-        const int any_hi = a.causal ? min(w.length, pos0 + token_hi + 1) : w.length;
-        const int all_hi = a.causal ? min(w.length, pos0 + token_lo + 1) : w.length;
-        const int any_lo = a.window > 0 ? max(0, pos0 + token_lo - a.window + 1) : 0;
-        const int all_lo = a.window > 0 ? max(0, pos0 + token_hi - a.window + 1) : 0;
-
         float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -250,11 +319,6 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel
         // 2t + 9. Each half is loaded again as soon as its product has used it.
         uint32_t xk[KV][2][4], xv[4][VB / 4];
         float ks = 0.f, vs = 1.f;
-        auto key_of = [&](int u) { return (w.unit0 + u) * UK + warp * 16; };
-        auto page_of = [&](int u) {
-            const int key = key_of(u);
-            return u < u1 && key < any_hi && key + 16 > any_lo ? table[key >> pl.page_shift] : -2;
-        };
         auto valid = [&](int page) {
             const bool have = unsigned(page) < unsigned(pl.pages);
             if (!have && page != -2 && lane == 0) atomicOr(a.status, kStatusPage);
@@ -291,7 +355,6 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel
             ks = pl.k_scale[ph];
             vs = pl.v_scale[ph];
         };
-        int page = page_of(u0), next_page = page_of(u0 + 1);
         bool have = valid(page);
         if (have) {
             load_k(u0, page);
@@ -468,8 +531,7 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel
         }
         if (split) {
             // blocks that hold a piece of this item: unit u lies in block floor(((u + 1) blocks - 1) / total)
-            const int b0 = int(((item_at + kFewItem + 1) * blocks - 1) / total);
-            const int b1 = int((item_end * blocks - 1) / total);
+            const int b0 = int(((item_at + kFewItem + 1) * blocks - 1) / total), b1 = int((item_end * blocks - 1) / total);
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -480,36 +542,7 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT>()) attend_few_kernel
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                const int64_t b0_start = total * b0 / blocks;
-                for (int e = tid; e < RT * (D / 4); e += W * 32) {
-                    const int r = e / (D / 4), d = e % (D / 4) * 4;
-                    if (r >= rows) continue;
-                    float top = ninf, sum = 0.f;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int b = b0; b <= b1; ++b) {
-                        const float *p = f.partial + int64_t(2 * b + (b == b0 && b0_start < item_at ? 1 : 0)) * SLOT;
-                        const float mk = __ldcg(p + RT * D + r), lk = __ldcg(p + RT * D + RT + r);
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + r * D + d));
-                        const float to = fmaxf(top, mk);
-                        const float fa = top == ninf ? (sum != sum ? 1.f : 0.f) : ex2(top - to);
-                        const float fb = mk == ninf ? (lk != lk ? 1.f : 0.f) : ex2(mk - to);
-                        acc.x = acc.x * fa + x.x * fb;
-                        acc.y = acc.y * fa + x.y * fb;
-                        acc.z = acc.z * fa + x.z * fb;
-                        acc.w = acc.w * fa + x.w * fb;
-                        sum = sum * fa + lk * fb;
-                        top = to;
-                    }
-                    const int q = tile * RT + r, token = q / a.group, hq = h * a.group + q - token * a.group;
-                    const float norm = sum == 0.f ? 0.f : 1.f / sum;
-                    Vec<T, 4> y;
-                    y.v[0] = from_f32<T>(acc.x * norm), y.v[1] = from_f32<T>(acc.y * norm);
-                    y.v[2] = from_f32<T>(acc.z * norm), y.v[3] = from_f32<T>(acc.w * norm);
-                    *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (w.first + token) * a.o_token + hq * a.o_head + d) = y;
-                    if (a.lse && d == 0)
-                        a.lse[int64_t(w.first + token) * (pl.heads * a.group) + hq] =
-                            sum == 0.f ? ninf : (top - kFewOffset + lg2(sum)) * 0.6931471805599453f;
-                }
+                join_pieces<T, D, NT, W>(f, b0, b1, share(total, b0, blocks) < item_at, h, tile, rows, w.first);
             }
         }
         at = min(item_end, end);
