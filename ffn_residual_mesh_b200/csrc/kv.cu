@@ -74,17 +74,25 @@ int check_table(const float *table, int rotary_dim, int max_positions, int head_
     return FFNRM_OK;
 }
 
+constexpr int kRotaryHeads = 4;
+
+template <typename T, bool INTERLEAVED, int VEC, int HEADS>
+void launch_rotary_t(const RotaryArgs &a, float sign, cudaStream_t st) {
+    const int64_t n = int64_t(a.tokens) * ((a.heads + HEADS - 1) / HEADS) * rotary_units<INTERLEAVED, VEC>(a.dim, a.rot);
+    rotary_kernel<T, INTERLEAVED, VEC, HEADS><<<unsigned((n + 255) / 256), 256, 0, st>>>(a, sign);
+}
+
 template <typename T, bool INTERLEAVED>
-void launch_rotary(const RotaryArgs &a, float sign, bool vec, cudaStream_t st) {
+void launch_rotary(const RotaryArgs &a, float sign, bool wide_rows, cudaStream_t st) {
     constexpr int N = 16 / int(sizeof(T));
-    const bool wide_rows = vec && rotary_fits<INTERLEAVED, N>(a.dim, a.rot);
-    const int units = wide_rows ? rotary_units<INTERLEAVED, N>(a.dim, a.rot) : rotary_units<INTERLEAVED, 1>(a.dim, a.rot);
-    const int64_t n = int64_t(a.tokens) * a.heads * units;
-    const unsigned grid = unsigned(std::min<int64_t>((n + 255) / 256, 1 << 20));
-    if (wide_rows)
-        rotary_kernel<T, INTERLEAVED, N><<<grid, 256, 0, st>>>(a, sign);
+    // few rows: one head to a thread, so that there are threads for every SM
+    const bool few = int64_t(a.tokens) * a.heads < 16384;
+    if (!wide_rows || !rotary_fits(INTERLEAVED, N, a.dim, a.rot, a.table))
+        launch_rotary_t<T, INTERLEAVED, 1, 1>(a, sign, st);
+    else if (few)
+        launch_rotary_t<T, INTERLEAVED, N, 1>(a, sign, st);
     else
-        rotary_kernel<T, INTERLEAVED, 1><<<grid, 256, 0, st>>>(a, sign);
+        launch_rotary_t<T, INTERLEAVED, N, kRotaryHeads>(a, sign, st);
 }
 
 }  // namespace
@@ -264,6 +272,7 @@ int ffnrm_rotary(const ffnrm_rows *x, const ffnrm_rows *y, int dtype, int tokens
     if (!positions || !aligned(positions, 4)) return fail(FFNRM_ERR_ARG, "null or misaligned positions");
     if (x->data == y->data && (x->token_stride != y->token_stride || x->head_stride != y->head_stride))
         return fail(FFNRM_ERR_ARG, "rotating in place needs equal strides");
+    if (int64_t(tokens) * heads * head_dim / 256 > 0x7fffffff) return fail(FFNRM_ERR_ARG, "tokens=%d are too many for one call", tokens);
     const RotaryArgs a{x->data, y->data, positions, table, x->token_stride, x->head_stride, y->token_stride, y->head_stride,
                        tokens, heads, head_dim, rotary_dim, max_positions};
     const bool vec = wide(*x, dtype) && wide(*y, dtype), inter = flags & FFNRM_ROTARY_INTERLEAVED;
@@ -387,8 +396,8 @@ int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     }
     const bool inter = flags & FFNRM_ROTARY_INTERLEAVED;
     const int N = 16 / int(type_size(dtype));
-    bool vec = wide(*k, dtype) && wide(*v, dtype) && (!has_q || (wide(*q, dtype) && wide(*q_out, dtype)));
-    if (has_q) vec = vec && rotary_dim % N == 0 && (inter || (rotary_dim / 2) % N == 0);
+    const bool vec = wide(*k, dtype) && wide(*v, dtype) && (!has_q || (wide(*q, dtype) && wide(*q_out, dtype))) &&
+                     (!table || rotary_fits(inter, 8, D, rotary_dim, table));
     AppendArgs a{};
     a.pool = layer_pool(kv, layer);
     a.batch = batch_view(batch);
@@ -402,10 +411,8 @@ int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
         a.q = q->data, a.q_token = q->token_stride, a.q_head = q->head_stride;
         a.q_out = q_out->data, a.o_token = q_out->token_stride, a.o_head = q_out->head_stride;
         a.q_heads = q_heads;
-        const int units = vec ? (inter ? rotary_units<true, 1>(D, 0) / N : (rotary_dim / 2 + D - rotary_dim) / N)
-                              : rotary_units<false, 1>(D, rotary_dim);
-        a.q_chunks = (units * q_heads + 255) / 256;
-        grid += int64_t(batch->rows) * a.q_chunks;
+        const int units = vec ? (inter ? D : D - rotary_dim / 2) / N : rotary_units<false, 1>(D, rotary_dim);
+        grid += (int64_t(batch->rows) * units * ((q_heads + kQueryHeads - 1) / kQueryHeads) + 255) / 256;
     }
     if (grid > 0x7fffffff) return fail(FFNRM_ERR_ARG, "rows=%d are too many for one call", batch->rows);
     DeviceGuard guard(kv->device);
@@ -425,16 +432,16 @@ int ffnrm_kv_read(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtyp
     if (rc || (rc = check_batch(kv, batch))) return rc;
     if (dtype < FFNRM_F16 || dtype > FFNRM_F32) return fail(FFNRM_ERR_ARG, "unknown element type %d", dtype);
     if (batch->rows == 0 || batch->seqs == 0) return FFNRM_OK;
-    if (!k || !v || !aligned(k, 16) || !aligned(v, 16)) return fail(FFNRM_ERR_ARG, "k and v must be 16-byte aligned");
+    if (!k || !v || !aligned(k, 32) || !aligned(v, 32)) return fail(FFNRM_ERR_ARG, "k and v must be 32-byte aligned");
     const ReadArgs a{layer_pool(kv, layer), batch_view(batch), k, v, kv->status};
     DeviceGuard guard(kv->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == FFNRM_F16)
-        read_kernel<__half><<<unsigned(batch->rows), 256, 0, st>>>(a);
+        read_kernel<__half><<<unsigned((batch->rows + 7) / 8), 256, 0, st>>>(a);
     else if (dtype == FFNRM_BF16)
-        read_kernel<__nv_bfloat16><<<unsigned(batch->rows), 256, 0, st>>>(a);
+        read_kernel<__nv_bfloat16><<<unsigned((batch->rows + 7) / 8), 256, 0, st>>>(a);
     else
-        read_kernel<float><<<unsigned(batch->rows), 256, 0, st>>>(a);
+        read_kernel<float><<<unsigned((batch->rows + 7) / 8), 256, 0, st>>>(a);
     KV_CUDA(cudaGetLastError());
     return FFNRM_OK;
 }

@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace ffnrm::kv {
 
 // Bits of the handle's status word, set by kernels that met data they cannot use.
@@ -98,6 +100,47 @@ template <typename T, int N>
 struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Vec {
     T v[N];
 };
+
+// N values to and from f32, two to an instruction where the type allows.
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Vec<T, N> &v, float *f) {
+    if constexpr (N % 2 == 0 && sizeof(T) == 2) {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const T2 p = *reinterpret_cast<const T2 *>(&v.v[i]);
+            float2 x;
+            if constexpr (std::is_same<T, __half>::value)
+                x = __half22float2(p);
+            else
+                x = __bfloat1622float2(p);
+            f[i] = x.x, f[i + 1] = x.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = to_f32(v.v[i]);
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> pack(const float *f) {
+    Vec<T, N> v;
+    if constexpr (N % 2 == 0 && sizeof(T) == 2) {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            T2 p;
+            if constexpr (std::is_same<T, __half>::value)
+                p = __floats2half2_rn(f[i], f[i + 1]);
+            else
+                p = __floats2bfloat162_rn(f[i], f[i + 1]);
+            *reinterpret_cast<T2 *>(&v.v[i]) = p;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v.v[i] = from_f32<T>(f[i]);
+    }
+    return v;
+}
 
 // The rotation of one pair in f32, every product and sum rounded by itself so that the
 // result does not depend on contraction: (a c - b s, b c + a s).

@@ -337,8 +337,8 @@ int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
                     const ffnrm_rows *v, const ffnrm_rows *q, const ffnrm_rows *q_out, int q_heads, const float *table,
                     int rotary_dim, int max_positions, int flags, void *stream);
 
-/* The batch's rows back from the cache: k, v [rows][kv_heads][head_dim] contiguous,
- * code * scale in `dtype`. Idle slots read as zeros. */
+/* The batch's rows back from the cache: k, v [rows][kv_heads][head_dim] contiguous and
+ * 32-byte aligned, code * scale in `dtype`. Idle slots read as zeros. */
 int ffnrm_kv_read(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, void *k, void *v, void *stream);
 
 /* Attention of a step's queries q [rows][q_heads][head_dim] (f16 or bf16; q_heads a multiple
