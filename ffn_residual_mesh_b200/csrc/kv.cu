@@ -109,7 +109,7 @@ struct ffnrm_kv {
     int *counters = nullptr;     // their arrivals, zero between calls
     int few_grid[2][2] = {};     // blocks by type and row tiles
     int32_t *scratch = nullptr;  // page lists of fork / compact
-    int32_t *src = nullptr, *dst = nullptr, *owner = nullptr, *list = nullptr, *rows = nullptr, *count = nullptr;
+    int32_t *src = nullptr, *dst = nullptr, *owner = nullptr, *list = nullptr, *count = nullptr;
 };
 
 namespace {
@@ -250,8 +250,17 @@ int launch_moves(ffnrm_kv *kv, const int32_t *src, const int32_t *dst, const int
                c.n_layers,  c.n_pages,   c.kv_heads,  page_bytes,  most, kv->status};
     const int64_t items = int64_t(most) * c.n_layers * 2 * ((page_bytes + kMoveChunk - 1) / kMoveChunk);
     const unsigned grid = unsigned(std::min<int64_t>(items, int64_t(kv->num_sms) * 8));
-    move_kernel<<<grid, 256, 0, st>>>(m);
-    KV_CUDA(cudaGetLastError());
+    // behind fork / compact as a dependent launch: it waits for the list itself
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = dim3(grid);
+    lc.blockDim = dim3(256);
+    lc.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = &attr;
+    lc.numAttrs = count ? 1 : 0;
+    KV_CUDA(cudaLaunchKernelEx(&lc, move_kernel, m));
     return FFNRM_OK;
 }
 
@@ -329,8 +338,7 @@ int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8
         return rc;
     }
     const size_t counters = size_t(*std::max_element(&kv->few_grid[0][0], &kv->few_grid[0][0] + 4));
-    const size_t ints = 4 * list + 4 * size_t(c.max_seqs) + 2 + counters;
-    const int bitmap = (c.n_pages + 31) / 32 * 4;
+    const size_t ints = 4 * list + 2 + counters;
     if (cudaMalloc(&kv->partial, floats * sizeof(float)) != cudaSuccess) {
         cudaGetLastError();
         delete kv;
@@ -346,13 +354,13 @@ int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8
     kv->dst = kv->src + list;
     kv->owner = kv->dst + list;
     kv->list = kv->owner + list;
-    kv->rows = kv->list + list;
-    kv->count = kv->rows + 4 * size_t(c.max_seqs);
+    kv->count = kv->list + list;
     kv->status = kv->count + 1;
     kv->counters = kv->status + 1;
+    // a bit for each of up to 2^20 pages, and 16 bytes for each of up to 4096 children
     cudaError_t e = cudaMemset(kv->scratch, 0, ints * sizeof(int32_t));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(bitmap, 1 << 17));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(bitmap, 1 << 17));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16);
     if (e == cudaSuccess) e = prepare_many<__half>(c.head_dim);
     if (e == cudaSuccess) e = prepare_many<__nv_bfloat16>(c.head_dim);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -489,8 +497,8 @@ int ffnrm_kv_fork(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, i
     DeviceGuard guard(kv->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const PageArgs a{tables, lengths, parents, extra, out_tables, out_lengths, info, kv->src, kv->dst, kv->count, kv->owner,
-                     kv->list, kv->rows, seqs, table_width, children, out_width, kv->cfg.n_pages, kv->page_shift, kv->status};
-    fork_kernel<<<1, kPageThreads, size_t(kv->cfg.n_pages + 31) / 32 * 4, st>>>(a);
+                     kv->list, seqs, table_width, children, out_width, kv->cfg.n_pages, kv->page_shift, kv->status};
+    fork_kernel<<<1, kPageThreads, size_t(kv->cfg.n_pages + 31) / 32 * 4 + size_t(children) * 16, st>>>(a);
     KV_CUDA(cudaGetLastError());
     if (children == 0) return FFNRM_OK;
     return launch_moves(kv, kv->src, kv->dst, kv->count, std::min(children, kv->cfg.n_pages), st);
@@ -507,8 +515,8 @@ int ffnrm_kv_compact(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths
     DeviceGuard guard(kv->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const PageArgs a{tables, lengths, nullptr, nullptr, out_tables, nullptr, info, kv->src, kv->dst, kv->count, kv->owner,
-                     kv->list, kv->rows, seqs, table_width, 0, table_width, kv->cfg.n_pages, kv->page_shift, kv->status};
-    compact_kernel<<<1, kPageThreads, size_t(kv->cfg.n_pages + 31) / 32 * 4, st>>>(a);
+                     kv->list, seqs, table_width, 0, table_width, kv->cfg.n_pages, kv->page_shift, kv->status};
+    compact_kernel<<<1, kPageThreads, size_t(kv->cfg.n_pages + 31) / 32 * 4 + size_t(seqs) * 4, st>>>(a);
     KV_CUDA(cudaGetLastError());
     return launch_moves(kv, kv->src, kv->dst, kv->count, kv->cfg.n_pages, st);
 }

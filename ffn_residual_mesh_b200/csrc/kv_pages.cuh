@@ -24,7 +24,6 @@ struct PageArgs {
     int32_t *info;                    // [4]: pages held, pages free, pages copied or moved, pages short
     int32_t *src, *dst, *count;       // the moves, for move_kernel
     int32_t *owner, *list;            // scratch, [pages] each
-    int32_t *rows;                    // scratch, [4][children]
     int seqs, width, children, out_width, pages, page_shift;
     int *status;
 };
@@ -61,12 +60,44 @@ __device__ __forceinline__ int block_or(int bits, int *shared) {
     return *shared;
 }
 
-// One block. Shared memory: a bit per page.
+// f(row, column, index) for every entry of a [rows][width] table, kPageBatch entries of a thread at a
+// time, so that their loads are under way together: get loads, put uses.
+constexpr int kPageBatch = 8;
+template <typename Index, typename Get, typename Put>
+__device__ __forceinline__ void for_entries_of(Index total, Index width, Get get, Put put) {
+    for (Index e0 = threadIdx.x; e0 < total; e0 += kPageThreads * kPageBatch) {
+        int v[kPageBatch], row[kPageBatch], col[kPageBatch];
+#pragma unroll
+        for (int i = 0; i < kPageBatch; ++i) {
+            const Index e = e0 + i * kPageThreads;
+            row[i] = int(e / width);
+            col[i] = int(e - Index(row[i]) * width);
+            if (e < total) v[i] = get(row[i], col[i], int64_t(e));
+        }
+#pragma unroll
+        for (int i = 0; i < kPageBatch; ++i) {
+            const Index e = e0 + i * kPageThreads;
+            if (e < total) put(row[i], col[i], int64_t(e), v[i]);
+        }
+    }
+}
+template <typename Get, typename Put>
+__device__ __forceinline__ void for_entries(int rows, int width, Get get, Put put) {
+    const int64_t total = int64_t(rows) * width;
+    if (total < (1 << 30))  // 64-bit divisions would take longer than the loads
+        for_entries_of<uint32_t>(uint32_t(total), uint32_t(width), get, put);
+    else
+        for_entries_of<int64_t>(total, width, get, put);
+}
+
+// One block. Shared memory: a bit per page, four integers per child. Bound by the latency of the
+// dependent loads (parent, length, table entry) and a dozen barriers.
 __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
     extern __shared__ uint32_t held[];
     __shared__ int flags;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int words = (a.pages + 31) / 32, P = 1 << a.page_shift, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int32_t *full = a.rows, *open = full + a.children, *need = open + a.children, *from = need + a.children;
+    int *full = reinterpret_cast<int *>(held + words), *open = full + a.children, *need = open + a.children, *from = need + a.children;
     for (int i = tid; i < words; i += kPageThreads) held[i] = 0;
     if (tid == 0) flags = 0;
     __syncthreads();
@@ -108,22 +139,25 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
         a.out_lengths[c] = length + grow;
     }
     block_or(bad, &flags);
-    // shared pages
+    // shared pages: a warp per child
     for (int c = warp; c < a.children; c += kPageThreads / 32) {
-        const int p = from[c], nf = full[c];
-        if (p < 0) continue;
+        const int nf = full[c];
+        const int32_t *row = a.tables + int64_t(max(0, from[c])) * a.width;
+        int32_t *out = a.out_tables + int64_t(c) * a.out_width;
+#pragma unroll 4
         for (int w = lane; w < nf; w += 32) {
-            int id = a.tables[int64_t(p) * a.width + w];
-            if (id >= 0 && id < a.pages)
+            int id = row[w];
+            if (id >= 0 && id < a.pages) {
                 atomicOr(&held[id >> 5], 1u << (id & 31));
-            else {
+            } else {
                 bad |= kStatusPage;
                 id = -1;
             }
-            a.out_tables[int64_t(c) * a.out_width + w] = id;
+            out[w] = id;
         }
-        if (lane == 0 && open[c] >= 0) atomicMin(&a.owner[open[c]], c);
     }
+    for (int c = tid; c < a.children; c += kPageThreads)
+        if (open[c] >= 0) atomicMin(&a.owner[open[c]], c);
     bad = block_or(bad, &flags);
     // who keeps an open page; decided before any of them is marked
     for (int c = tid; c < a.children; c += kPageThreads) {
@@ -165,6 +199,7 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
         }
     }
     __syncthreads();
+    int *count = from;  // from here on: a child's new pages
     for (int c = c0; c < c1; ++c) {
         const int n = need[c];
         if (open[c] >= 0 && full[c] >= 0 && !refuse) {
@@ -173,6 +208,7 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
             ++copy_at;
         }
         need[c] = offset;
+        count[c] = n;
         offset += n;
         if (refuse) a.out_lengths[c] = 0;
     }
@@ -188,46 +224,51 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
     // the rest of each row: the open page or its copy, new pages, none
     for (int c = warp; c < a.children; c += kPageThreads / 32) {
         const bool keep = full[c] < 0;
-        const int nf = full[c] & 0x7fffffff;
-        const int end = (a.out_lengths[c] + P - 1) >> a.page_shift;
+        const int nf = full[c] & 0x7fffffff, first = nf + (keep ? 1 : 0), n = count[c], at = need[c];
+        int32_t *out = a.out_tables + int64_t(c) * a.out_width;
+#pragma unroll 4
         for (int w = refuse ? lane : nf + lane; w < a.out_width; w += 32) {
-            int id = -1;
-            if (!refuse && w < end) id = keep ? (w == nf ? open[c] : a.list[need[c] + w - nf - 1]) : a.list[need[c] + w - nf];
-            a.out_tables[int64_t(c) * a.out_width + w] = id;
+            const int i = w - first;
+            const int fresh = __ldcg(a.list + max(0, min(at + i, a.pages - 1)));
+            out[w] = refuse ? -1 : i < 0 ? open[c] : i < n ? fresh : -1;
         }
     }
 }
 
-// One block. Shared memory: a bit per page.
+// One block. Shared memory: a bit per page, an integer per sequence.
 __global__ void __launch_bounds__(kPageThreads) compact_kernel(PageArgs a) {
     extern __shared__ uint32_t held[];
     __shared__ int flags;
-    const int words = (a.pages + 31) / 32, P = 1 << a.page_shift, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int words = (a.pages + 31) / 32, P = 1 << a.page_shift, tid = threadIdx.x;
     for (int i = tid; i < words; i += kPageThreads) held[i] = 0;
     if (tid == 0) flags = 0;
     __syncthreads();
     int bad = 0;
-    for (int s = warp; s < a.seqs; s += kPageThreads / 32) {
-        int length = a.lengths[s];
-        if (length < 0 || length > (int64_t(a.width) << a.page_shift)) {
-            bad |= kStatusLength;
-            length = 0;
-        }
-        const int n = (length + P - 1) >> a.page_shift;
-        for (int w = lane; w < n; w += 32) {
-            const int id = a.tables[int64_t(s) * a.width + w];
+    // pages of each sequence; 0 for a length that its row cannot hold
+    int *full = reinterpret_cast<int *>(held + words);
+    for (int s = tid; s < a.seqs; s += kPageThreads) {
+        const int length = a.lengths[s];
+        const bool fits = length >= 0 && length <= (int64_t(a.width) << a.page_shift);
+        full[s] = fits ? (length + P - 1) >> a.page_shift : 0;
+        if (!fits) bad |= kStatusLength;
+    }
+    __syncthreads();
+    for_entries(
+        a.seqs, a.width, [&](int, int, int64_t e) { return a.tables[e]; },
+        [&](int s, int w, int64_t, int id) {
+            if (w >= full[s]) return;
             if (id >= 0 && id < a.pages)
                 atomicOr(&held[id >> 5], 1u << (id & 31));
             else
                 bad |= kStatusPage;
-        }
-    }
+        });
     bad = block_or(bad, &flags);
     const int per = (words + kPageThreads - 1) / kPageThreads, w0 = tid * per, w1 = min(words, w0 + per);
     int mine = 0, used;
     for (int w = w0; w < w1; ++w) mine += __popc(held[w]);
     int before = block_scan(mine, used);  // held pages below this thread's words
-    // holes below `used` in order, then the held pages at or above it
+    // holes below `used`, in order
     for (int w = w0; w < w1; ++w) {
         const int inside = used - w * 32;
         if (inside <= 0) break;
@@ -237,28 +278,25 @@ __global__ void __launch_bounds__(kPageThreads) compact_kernel(PageArgs a) {
         for (; b; b &= b - 1) a.list[rank++] = w * 32 + __ffs(b) - 1;
     }
     __syncthreads();
-    // held pages below `used`, so that those above can be ranked
-    int low = 0, low_total, high = 0, high_total;
+    // the held pages at or above `used`, in order
+    int high = 0, high_total;
     for (int w = w0; w < w1; ++w) {
         const int inside = used - w * 32;
         const uint32_t lowmask = inside <= 0 ? 0u : inside >= 32 ? 0xffffffffu : (1u << inside) - 1u;
-        low += __popc(held[w] & lowmask);
         high += __popc(held[w] & ~lowmask);
     }
-    block_scan(low, low_total);
     int rank = block_scan(high, high_total);
     for (int w = w0; w < w1; ++w) {
         const int inside = used - w * 32;
         const uint32_t lowmask = inside <= 0 ? 0u : inside >= 32 ? 0xffffffffu : (1u << inside) - 1u;
-        for (uint32_t b = held[w] & ~lowmask; b; b &= b - 1) {
-            const int id = w * 32 + __ffs(b) - 1, to = a.list[rank];
-            a.owner[id] = to;
-            if (!bad) {
-                a.src[rank] = id;
-                a.dst[rank] = to;
-            }
-            ++rank;
-        }
+        for (uint32_t b = held[w] & ~lowmask; b; b &= b - 1) a.src[rank++] = w * 32 + __ffs(b) - 1;
+    }
+    __syncthreads();
+    // the k-th held page above goes to the k-th hole below
+    for (int k = tid; k < high_total; k += kPageThreads) {
+        const int to = __ldcg(a.list + k);
+        a.owner[__ldcg(a.src + k)] = to;
+        a.dst[k] = to;
     }
     if (tid == 0) {
         a.info[kInfoUsed] = used;
@@ -270,18 +308,13 @@ __global__ void __launch_bounds__(kPageThreads) compact_kernel(PageArgs a) {
     }
     __syncthreads();
     // bad tables: nothing moves and the rows are handed on as they are
-    for (int s = warp; s < a.seqs; s += kPageThreads / 32) {
-        const int length = a.lengths[s];
-        const int n = bad ? a.width : (length + P - 1) >> a.page_shift;
-        for (int w = lane; w < a.width; w += 32) {
-            int id = -1;
-            if (w < n) {
-                id = a.tables[int64_t(s) * a.width + w];
-                if (!bad && id >= used) id = __ldcg(&a.owner[id]);
-            }
-            a.out_tables[int64_t(s) * a.width + w] = id;
-        }
-    }
+    for_entries(
+        a.seqs, a.width,
+        [&](int, int, int64_t e) { return a.tables[e]; },
+        [&](int s, int w, int64_t e, int id) {
+            if (!bad) id = w >= full[s] ? -1 : id >= used ? __ldcg(&a.owner[id]) : id;
+            a.out_tables[e] = id;
+        });
 }
 
 struct MoveArgs {
@@ -293,39 +326,47 @@ struct MoveArgs {
     int *status;
 };
 
-constexpr int kMoveChunk = 16384;
+constexpr int kMoveChunk = 32768, kMoveLoads = kMoveChunk / 16 / 256;
 
-// Copies every listed page in every layer, kMoveChunk bytes of codes per block step.
+// Copies every listed page in every layer, kMoveChunk bytes of codes per block step. Bound by reading and
+// writing them once: eight 16-byte loads under way per thread, the next step's page ids read ahead.
 __global__ void __launch_bounds__(256) move_kernel(MoveArgs a) {
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the list is the kernel's before
     const int moves = a.count ? min(*a.count, a.most) : a.most, chunks = (a.page_bytes + kMoveChunk - 1) / kMoveChunk;
-    const int64_t items = int64_t(moves) * a.layers * 2 * chunks;
-    for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
-        const int chunk = int(i % chunks);
-        int64_t r = i / chunks;
-        const int kv = int(r & 1);
-        r >>= 1;
-        const int layer = int(r % a.layers), m = int(r / a.layers);
-        const int src = a.src[m], dst = a.dst[m];
-        if (src < 0 || src >= a.pages || dst < 0 || dst >= a.pages) {
-            if (threadIdx.x == 0) atomicOr(a.status, kStatusPage);
-            continue;
-        }
-        const int64_t from = int64_t(layer) * a.pages + src, to = int64_t(layer) * a.pages + dst;
-        int8_t *codes = kv ? a.v_codes : a.k_codes;
-        const uint4 *x = reinterpret_cast<const uint4 *>(codes + from * a.page_bytes + int64_t(chunk) * kMoveChunk);
-        uint4 *y = reinterpret_cast<uint4 *>(codes + to * a.page_bytes + int64_t(chunk) * kMoveChunk);
-        const int n = min(kMoveChunk, a.page_bytes - chunk * kMoveChunk) / 16;
-        uint4 v[4];
+    const int per_move = a.layers * 2 * chunks;
+    const int64_t items = int64_t(moves) * per_move;
+    int64_t i = blockIdx.x;
+    if (i >= items) return;
+    int m = int(i / per_move);
+    int src = a.src[m], dst = a.dst[m];
+    while (true) {
+        const int part = int(i - int64_t(m) * per_move), chunk = part % chunks, kv = part / chunks & 1, layer = part / chunks >> 1;
+        const int64_t next = i + gridDim.x;
+        const bool more = next < items;
+        const int next_m = more ? int(next / per_move) : m;
+        const int next_src = a.src[next_m], next_dst = a.dst[next_m];
+        if (unsigned(src) < unsigned(a.pages) && unsigned(dst) < unsigned(a.pages)) {
+            const int64_t from = int64_t(layer) * a.pages + src, to = int64_t(layer) * a.pages + dst;
+            int8_t *codes = kv ? a.v_codes : a.k_codes;
+            const uint4 *x = reinterpret_cast<const uint4 *>(codes + from * a.page_bytes + int64_t(chunk) * kMoveChunk);
+            uint4 *y = reinterpret_cast<uint4 *>(codes + to * a.page_bytes + int64_t(chunk) * kMoveChunk);
+            const int n = min(kMoveChunk, a.page_bytes - chunk * kMoveChunk) / 16;
+            uint4 v[kMoveLoads];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (int(threadIdx.x) + j * 256 < n) v[j] = x[threadIdx.x + j * 256];
+            for (int j = 0; j < kMoveLoads; ++j)
+                if (int(threadIdx.x) + j * 256 < n) v[j] = x[threadIdx.x + j * 256];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (int(threadIdx.x) + j * 256 < n) y[threadIdx.x + j * 256] = v[j];
-        if (chunk == 0) {
-            float *scale = kv ? a.v_scale : a.k_scale;
-            for (int h = threadIdx.x; h < a.heads; h += 256) scale[to * a.heads + h] = scale[from * a.heads + h];
+            for (int j = 0; j < kMoveLoads; ++j)
+                if (int(threadIdx.x) + j * 256 < n) y[threadIdx.x + j * 256] = v[j];
+            if (chunk == 0) {
+                float *scale = kv ? a.v_scale : a.k_scale;
+                for (int h = threadIdx.x; h < a.heads; h += 256) scale[to * a.heads + h] = scale[from * a.heads + h];
+            }
+        } else if (threadIdx.x == 0) {
+            atomicOr(a.status, kStatusPage);
         }
+        if (!more) return;
+        i = next, m = next_m, src = next_src, dst = next_dst;
     }
 }
 
