@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 #include <new>
 
 #include "kv_append.cuh"
@@ -95,6 +96,14 @@ void launch_rotary(const RotaryArgs &a, float sign, bool wide_rows, cudaStream_t
         launch_rotary_t<T, INTERLEAVED, N, kRotaryHeads>(a, sign, st);
 }
 
+// What a device needs once: the blocks of each few-rows variant that it holds (by type, head dim and row
+// tiles) and the workspace of partials for them.
+struct DeviceSetup {
+    bool done = false;
+    int sms = 0, grid[2][3][2] = {};
+    size_t floats[3] = {};
+};
+
 }  // namespace
 
 struct ffnrm_kv {
@@ -104,11 +113,11 @@ struct ffnrm_kv {
     int8_t *k_codes = nullptr, *v_codes = nullptr;
     float *k_scale = nullptr, *v_scale = nullptr;
     int num_sms = 148;
+    const DeviceSetup *setup = nullptr;
     int *status = nullptr;       // what kernels could not use, kStatus* bits
     float *partial = nullptr;    // pieces of attention items cut between blocks
     int *counters = nullptr;     // their arrivals, zero between calls
-    int few_grid[2][2] = {};     // blocks by type and row tiles
-    int32_t *scratch = nullptr;  // page lists of fork / compact
+    void *scratch = nullptr;     // the handle's memory: all of the above and the page lists of fork / compact
     int32_t *src = nullptr, *dst = nullptr, *owner = nullptr, *list = nullptr, *count = nullptr;
 };
 
@@ -185,23 +194,48 @@ int with_few(int dtype, int dim, int nt, F f) {
 #undef FEW
 }
 
-// Prepares every variant and sizes the workspace of partials: one block per free slot of the GPU.
-int prepare_few(ffnrm_kv *kv, size_t &floats) {
-    int rc = FFNRM_OK;
+int dim_index(int dim) { return dim == 64 ? 0 : dim == 128 ? 1 : 2; }
+
+template <typename T>
+cudaError_t prepare_many() {
+    cudaError_t e = cudaFuncSetAttribute(attend_many_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<64>::SMEM);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(attend_many_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<128>::SMEM);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(attend_many_kernel<T, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<256>::SMEM);
+    return e;
+}
+
+int device_setup(int device, const DeviceSetup *&out) {
+    static std::mutex lock;
+    static DeviceSetup table[64];
+    if (device >= 64) return fail(FFNRM_ERR_ARG, "device %d beyond the supported 64", device);
+    const std::lock_guard<std::mutex> hold(lock);
+    DeviceSetup &d = table[device];
+    out = &d;
+    if (d.done) return FFNRM_OK;
+    KV_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device));
     for (int dtype : {FFNRM_F16, FFNRM_BF16})
-        for (int nt : {1, 2}) {
-            rc = with_few(dtype, kv->cfg.head_dim, nt, [&](auto kernel, int smem, int slot) {
-                int per_sm = 0;
-                KV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-                KV_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kFewWarps * 32, smem));
-                const int grid = std::max(1, per_sm) * kv->num_sms;
-                kv->few_grid[dtype][nt - 1] = grid;
-                floats = std::max(floats, size_t(2) * grid * slot);
-                return int(FFNRM_OK);
-            });
-            if (rc) return rc;
-        }
-    return rc;
+        for (int dim : {64, 128, 256})
+            for (int nt : {1, 2}) {
+                const int rc = with_few(dtype, dim, nt, [&](auto kernel, int smem, int slot) {
+                    int per_sm = 0;
+                    KV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+                    KV_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kFewWarps * 32, smem));
+                    const int i = dim_index(dim), grid = std::max(1, per_sm) * d.sms;
+                    d.grid[dtype][i][nt - 1] = grid;
+                    d.floats[i] = std::max(d.floats[i], size_t(2) * grid * slot);
+                    return int(FFNRM_OK);
+                });
+                if (rc) return rc;
+            }
+    KV_CUDA(prepare_many<__half>());
+    KV_CUDA(prepare_many<__nv_bfloat16>());
+    // a bit for each of up to 2^20 pages, and 16 bytes for each of up to 4096 sequences
+    KV_CUDA(cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16));
+    KV_CUDA(cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16));
+    d.done = true;
+    return FFNRM_OK;
 }
 
 int launch_few(ffnrm_kv *kv, const AttendArgs &a, int dtype, int most_rows, cudaStream_t st) {
@@ -210,7 +244,7 @@ int launch_few(ffnrm_kv *kv, const AttendArgs &a, int dtype, int most_rows, cuda
     const int nt = rows > 8 ? 2 : 1;
     const FewArgs f{a, kv->partial, kv->counters, kFewMinUnits, most_rows};
     return with_few(dtype, kv->cfg.head_dim, nt, [&](auto kernel, int smem, int) {
-        kernel<<<unsigned(kv->few_grid[dtype][nt - 1]), kFewWarps * 32, smem, st>>>(f);
+        kernel<<<unsigned(kv->setup->grid[dtype][dim_index(kv->cfg.head_dim)][nt - 1]), kFewWarps * 32, smem, st>>>(f);
         KV_CUDA(cudaGetLastError());
         return int(FFNRM_OK);
     });
@@ -221,15 +255,6 @@ int launch_many_t(ffnrm_kv *kv, const ManyArgs &m, cudaStream_t st) {
     attend_many_kernel<T, D><<<unsigned(m.slots) * unsigned(kv->cfg.kv_heads), Many<D>::THREADS, Many<D>::SMEM, st>>>(m);
     KV_CUDA(cudaGetLastError());
     return FFNRM_OK;
-}
-
-template <typename T>
-cudaError_t prepare_many(int dim) {
-    if (dim == 64)
-        return cudaFuncSetAttribute(attend_many_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<64>::SMEM);
-    if (dim == 128)
-        return cudaFuncSetAttribute(attend_many_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<128>::SMEM);
-    return cudaFuncSetAttribute(attend_many_kernel<T, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<256>::SMEM);
 }
 
 int launch_many(ffnrm_kv *kv, const AttendArgs &a, int dtype, int few_rows, bool alone, cudaStream_t st) {
@@ -329,44 +354,36 @@ int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8
         return fail(FFNRM_ERR_CUDA, "no CUDA device %d", device);
     }
     DeviceGuard guard(device);
-    cudaDeviceGetAttribute(&kv->num_sms, cudaDevAttrMultiProcessorCount, device);
-    const size_t list = size_t(std::max(c.n_pages, c.max_seqs));
-    size_t floats = 0;
-    int rc = prepare_few(kv, floats);
+    int rc = device_setup(device, kv->setup);
     if (rc) {
         delete kv;
         return rc;
     }
-    const size_t counters = size_t(*std::max_element(&kv->few_grid[0][0], &kv->few_grid[0][0] + 4));
-    const size_t ints = 4 * list + 2 + counters;
-    if (cudaMalloc(&kv->partial, floats * sizeof(float)) != cudaSuccess) {
+    kv->num_sms = kv->setup->sms;
+    // one allocation: page lists, the words that must start as zero (status, arrivals), partials
+    const size_t list = size_t(std::max(c.n_pages, c.max_seqs)), lists = 4 * list * sizeof(int32_t);
+    int most = 1;
+    for (int dtype : {FFNRM_F16, FFNRM_BF16})
+        for (int nt : {0, 1}) most = std::max(most, kv->setup->grid[dtype][dim_index(c.head_dim)][nt]);
+    const size_t zeros = (size_t(most) + 2) * sizeof(int), partial_at = (lists + zeros + 255) / 256 * 256;
+    const size_t bytes = partial_at + kv->setup->floats[dim_index(c.head_dim)] * sizeof(float);
+    if (cudaMalloc(&kv->scratch, bytes) != cudaSuccess) {
         cudaGetLastError();
         delete kv;
-        return fail(FFNRM_ERR_NOMEM, "cudaMalloc of %zu bytes failed", floats * sizeof(float));
+        return fail(FFNRM_ERR_NOMEM, "cudaMalloc of %zu bytes failed", bytes);
     }
-    if (cudaMalloc(&kv->scratch, ints * sizeof(int32_t)) != cudaSuccess) {
-        cudaGetLastError();
-        cudaFree(kv->partial);
-        delete kv;
-        return fail(FFNRM_ERR_NOMEM, "cudaMalloc of %zu bytes failed", ints * sizeof(int32_t));
-    }
-    kv->src = kv->scratch;
+    kv->src = static_cast<int32_t *>(kv->scratch);
     kv->dst = kv->src + list;
     kv->owner = kv->dst + list;
     kv->list = kv->owner + list;
     kv->count = kv->list + list;
     kv->status = kv->count + 1;
     kv->counters = kv->status + 1;
-    // a bit for each of up to 2^20 pages, and 16 bytes for each of up to 4096 children
-    cudaError_t e = cudaMemset(kv->scratch, 0, ints * sizeof(int32_t));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16);
-    if (e == cudaSuccess) e = prepare_many<__half>(c.head_dim);
-    if (e == cudaSuccess) e = prepare_many<__nv_bfloat16>(c.head_dim);
-    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    kv->partial = reinterpret_cast<float *>(static_cast<char *>(kv->scratch) + partial_at);
+    cudaError_t e = cudaMemset(kv->count, 0, zeros);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // the calls' streams may not be ordered behind it
     if (e != cudaSuccess) {
         cudaFree(kv->scratch);
-        cudaFree(kv->partial);
         delete kv;
         return fail(FFNRM_ERR_CUDA, "creating the cache failed: %s", cudaGetErrorString(e));
     }
@@ -378,7 +395,6 @@ int ffnrm_kv_destroy(ffnrm_kv *kv) {
     if (!kv) return FFNRM_OK;
     DeviceGuard guard(kv->device);
     cudaFree(kv->scratch);  // waits for the device
-    cudaFree(kv->partial);
     cudaGetLastError();
     delete kv;
     return FFNRM_OK;
