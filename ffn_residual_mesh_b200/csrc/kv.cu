@@ -168,8 +168,6 @@ void launch_append(const AppendArgs &a, bool vec, bool interleaved, unsigned gri
 }
 
 constexpr int kFewWarps = 8, kFewMinUnits = 1;
-// Sequences with more query rows (tokens x group) than this take the tcgen05 kernel.
-constexpr int kFewRows = 64;
 
 // f(kernel, dynamic shared memory, floats of one partial) of the variant for rows of type T,
 // head dim D and NT tiles of eight rows.
@@ -236,6 +234,14 @@ int device_setup(int device, const DeviceSetup *&out) {
     KV_CUDA(cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16));
     d.done = true;
     return FFNRM_OK;
+}
+
+// Sequences with more query rows (tokens x group) than this take the tcgen05 kernel. It has one block for 256
+// rows of a kv head over all keys, the few-rows kernel splits the keys: where the blocks fill the GPU
+// the first is as fast from 64 rows on (16 sequences of up to 128 tokens x 8: 109 us, 146 with 256
+// here), where they do not the second up to 256 (2 sequences of up to 32 x 8 over 16k keys: 194 us, 281).
+int few_rows(const ffnrm_kv *kv, const ffnrm_kv_batch *batch, int group) {
+    return int64_t(batch->rows) * group * kv->cfg.kv_heads < int64_t(256) * kv->num_sms ? 256 : 64;
 }
 
 int launch_few(ffnrm_kv *kv, const AttendArgs &a, int dtype, int most_rows, cudaStream_t st) {
@@ -492,10 +498,11 @@ int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     DeviceGuard guard(kv->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Without starts every sequence has one token; with them the device knows which kernel a sequence takes.
-    const bool can_be_many = batch->starts && int64_t(batch->rows) * a.group > kFewRows;
+    const int most = few_rows(kv, batch, a.group);
+    const bool can_be_many = batch->starts && int64_t(batch->rows) * a.group > most;
     const bool only_many = can_be_many && batch->seqs == 1;
-    if (!only_many && (rc = launch_few(kv, a, dtype, can_be_many ? kFewRows : 0x7fffffff, st))) return rc;
-    return can_be_many ? launch_many(kv, a, dtype, only_many ? 0 : kFewRows, only_many, st) : FFNRM_OK;
+    if (!only_many && (rc = launch_few(kv, a, dtype, can_be_many ? most : 0x7fffffff, st))) return rc;
+    return can_be_many ? launch_many(kv, a, dtype, only_many ? 0 : most, only_many, st) : FFNRM_OK;
 }
 
 int ffnrm_kv_fork(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, int seqs, int table_width,

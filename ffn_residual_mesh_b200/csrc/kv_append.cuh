@@ -128,7 +128,7 @@ constexpr int kKept = 2;        // rows (twice 8 channels) that a thread keeps b
 // Blocks [0, slots * heads * 2): one (page, head, K or V) each. The rest: rows of q, rotated to
 // q_out, in runs of 256 units.
 template <typename T, bool VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
     const Pool &pl = a.pool;
     const int items = a.slots * pl.heads * 2;
     const int P = pl.page_tokens, D = pl.dim;
