@@ -491,6 +491,7 @@ int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     if (!wide(*q, dtype) || !wide(*out, dtype))
         return fail(FFNRM_ERR_ARG, "q and out rows must be 16-byte aligned");
     if (!aligned(lse, 4)) return fail(FFNRM_ERR_ARG, "lse must be 4-byte aligned");
+    window = std::min(window, 1 << 30);  // no sequence is longer; keeps position - window in 32 bits
     const AttendArgs a{layer_pool(kv, layer), batch_view(batch), q->data, out->data, lse, q->token_stride, q->head_stride,
                        out->token_stride, out->head_stride, q_heads / kv->cfg.kv_heads, scale, causal, window, kv->status};
     if (int64_t(batch->rows) * a.group > 0x7fffffff / 2)

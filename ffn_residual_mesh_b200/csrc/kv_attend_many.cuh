@@ -13,6 +13,11 @@
 // With two row tiles the tensor cores work on one while the other's softmax runs. MMAs of one
 // thread execute in order, so S of the next key tile may be written over P right behind the product
 // that reads it.
+//
+// Per 128 keys and 256 rows the products need 2048 cycles and the exponentials left to the MUFU 1536; the
+// loop takes 4300, the chain S - softmax - P - products with its hand-overs (116 cycles each) being
+// longer than either. Measured: 8192-token prompt, 32/8 heads x 128, causal: 596-620 us, 890-920
+// TFLOP/s (55% of the measured GEMM burst); 4096 tokens at head dim 256: 347 us.
 #pragma once
 
 #include <type_traits>

@@ -333,7 +333,7 @@ def test_attend_several_tokens(cuda, D, P, new, lengths):
         check_attend(cuda, new, lengths, H, G, D, P, dtype, seed=len(new) + D, strided=G == 5)
 
 
-@pytest.mark.parametrize("window", [1, 7, 16, 100, 128, 5000])
+@pytest.mark.parametrize("window", [1, 7, 16, 100, 128, 5000, 2 ** 31 - 1])
 def test_attend_window(cuda, window):
     check_attend(cuda, [1] * 4, [1, 90, 1500, 128], 2, 4, 128, 16, seed=window, window=window, with_starts=False)
     check_attend(cuda, [200, 3, 128], [333, 500, 128], 2, 4, 128, 32, seed=window, window=window)
@@ -615,6 +615,40 @@ def test_compact_unusable_tables_are_handed_on(cuda):
     with pytest.raises(RuntimeError):
         cache.check()
     assert out.tolist() == rows and info[2] == 0
+
+
+def test_fork_and_compact_in_a_graph(cuda):
+    """The page moves launch as dependents of the table kernels: the same inside a capture."""
+    import torch
+    import kv_reference as ref
+    from ffn_residual_mesh_b200.graphs import StepGraph
+    P = 16
+    cache = make_cache(cuda, 60, 2, 64, P, layers=2)
+    rows, lengths = [[40, 3, 59, -1, -1], [50, 7, -1, -1, -1]], [40, 20]
+    tables, lens = ints(rows, cuda), ints(lengths, cuda)
+    parents, extra = ints([0, 1, 0], cuda), ints([1, 1, 1], cuda)
+    t2, l2 = torch.empty(3, 5, dtype=torch.int32, device=cuda), torch.empty(3, dtype=torch.int32, device=cuda)
+    t3, info, info3 = torch.empty_like(t2), ints([0] * 4, cuda), ints([0] * 4, cuda)
+
+    def step():
+        cache.fork(tables, lens, parents, extra, out_tables=t2, out_lengths=l2, info=info)
+        cache.compact(t2, l2, out_tables=t3, info=info3)
+
+    graph = StepGraph(step)
+    parents.copy_(ints([1, 0, 1], cuda))
+    before = cache.k_codes.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    cache.check()
+    want, want_len, copies = ref.fork(rows, lengths, [1, 0, 1], [1, 1, 1], 60, P, 5)
+    assert t2.tolist() == want and l2.tolist() == want_len
+    packed, move = ref.compact(want, want_len, P)
+    assert t3.tolist() == packed
+    for pairs in (copies, move.items()):
+        for src, dst in pairs:
+            before[:, dst] = before[:, src]
+    assert torch.equal(cache.k_codes, before)
+    graph.close()
 
 
 def test_copy_pages(cuda):
