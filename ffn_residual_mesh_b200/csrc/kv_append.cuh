@@ -106,21 +106,19 @@ __device__ __forceinline__ void load_channels(const T *x, int d0, const float *t
     }
 }
 
-// Eight codes rint(x / s), |x| <= 127 s. x times 1 / s is within 127 * 2^-22 of the quotient, so it rounds to
-// the same integer unless it lies that near to a half; only then are the quotients divided out. The
-// rounding is the addition of 1.5 * 2^23, whose sum has the integer in its low byte.
+// Eight codes rint(x / s), |x| <= 127 s, inv = 1 / s rounded to nearest. The quotient is rounded as IEEE
+// division rounds it, by Markstein's correction: the remainder of a quotient within one ulp is exact in
+// a fused multiply-add, and adding it times inv rounds correctly; the first of the two steps brings x inv
+// within that ulp. (Ties are common: bf16 values over a bf16 maximum hit a half exactly once in some two
+// hundred.) The rounding is the addition of 1.5 * 2^23, whose sum has the integer in its low byte.
 __device__ __forceinline__ uint2 quantise(const float (&f)[8], float s, float inv) {
     uint32_t t[8];
-    float off = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float y = f[i] * inv, z = __fadd_rn(y, 12582912.f);
-        off = fmaxf(off, fabsf(__fsub_rn(y, __fsub_rn(z, 12582912.f))));
-        t[i] = __float_as_uint(z);
-    }
-    if (off > 0.4999f) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = __float_as_uint(__fadd_rn(__fdiv_rn(f[i], s), 12582912.f));
+        float y = f[i] * inv;
+        y = fmaf(fmaf(-y, s, f[i]), inv, y);
+        y = fmaf(fmaf(-y, s, f[i]), inv, y);
+        t[i] = __float_as_uint(__fadd_rn(y, 12582912.f));
     }
     return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
                       __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));

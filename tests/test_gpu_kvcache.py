@@ -217,6 +217,14 @@ def test_append_non_finite_values_mark_their_block(cuda):
     assert torch.isnan(cache.k_scale[1]).any() and torch.isnan(cache.v_scale[1]).any()
 
 
+@pytest.mark.parametrize("scale", [1.0, 3e-9, 1e-14, 7e-38, 1e30, 3e38 / 9])
+def test_append_quotients_of_every_size(cuda, scale):
+    """Values from the smallest to the largest: the codes are the IEEE quotients' still."""
+    check_append(cuda, [64, 40], [0, 9], 2, 64, 32, "f32", seed=11, spread=scale)
+    if scale in (1.0, 1e30):
+        check_append(cuda, [300, 200], [5, 0], 4, 128, 64, "bf16", seed=12, spread=scale)  # ties
+
+
 def test_append_token_by_token_stays_near_the_values(cuda):
     """200 single appends: a code's error is at most half a step at its own write and half a
     step of the then larger scale at each growth; with growths of a fixed ratio 1.05 or more
