@@ -340,6 +340,7 @@ int ffnrm_kv_create(ffnrm_kv **out, int device, const ffnrm_kv_config *cfg, int8
         return fail(FFNRM_ERR_ARG, "head_dim=%d must be 64, 128 or 256", c.head_dim);
     if (c.page_tokens != 16 && c.page_tokens != 32 && c.page_tokens != 64 && c.page_tokens != 128)
         return fail(FFNRM_ERR_ARG, "page_tokens=%d must be 16, 32, 64 or 128", c.page_tokens);
+    static_assert(kFewSeqs == 4096, "the few-rows kernel keeps a sum for each 32 sequences");
     if (c.max_seqs <= 0 || c.max_seqs > 4096) return fail(FFNRM_ERR_ARG, "max_seqs=%d outside [1, 4096]", c.max_seqs);
     if (!k_codes || !v_codes || !k_scale || !v_scale) return fail(FFNRM_ERR_ARG, "null pool");
     if (!aligned(k_codes, 16) || !aligned(v_codes, 16) || !aligned(k_scale, 4) || !aligned(v_scale, 4))

@@ -29,6 +29,7 @@
 namespace ffnrm::kv {
 
 constexpr float kFewOffset = 7.f, kFewStep = 8.f;
+constexpr int kFewSeqs = 4096;  // most sequences of a call
 
 __device__ __forceinline__ uint32_t hsub2_bits(uint32_t a, uint32_t b) {
     const __half2 r = __hsub2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
@@ -186,47 +187,51 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT, W>()) attend_few_ker
 
     zero_loose_rows<T>(a);
     // This block's stretch of the line of units.
-    int64_t total = 0, mine = 0;
-    for (int s0 = 0; s0 < a.batch.seqs; s0 += 32) {
-        int64_t u = 0;
-        if (s0 + lane < a.batch.seqs) {
-            const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
-            u = int64_t(w.span()) * w.tiles * pl.heads;
-        }
-        mine = u;
+    // (sequences in runs of 32; above one run the warps share them out and leave each run's sum)
+    __shared__ int64_t run_sum[kFewSeqs / 32];
+    const int runs = (a.batch.seqs + 31) / 32;
+    auto span_of = [&](int s) -> int64_t {
+        if (s >= a.batch.seqs) return 0;
+        const SeqWork w = seq_work<UK, RT>(a, s, f.most_rows);
+        return int64_t(w.span()) * w.tiles * pl.heads;
+    };
+    auto warp_sum = [&](int64_t u) {
         for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-        total += u;
+        return u;
+    };
+    int64_t total = 0, mine = 0;
+    if (runs <= 1) {
+        mine = span_of(lane);
+        total = warp_sum(mine);
+    } else {
+        for (int r = warp; r < runs; r += W) {
+            const int64_t sum = warp_sum(span_of(r * 32 + lane));
+            if (lane == 0) run_sum[r] = sum;
+        }
+        __syncthreads();
+        for (int r = lane; r < runs; r += 32) total += run_sum[r];
+        total = warp_sum(total);
     }
     if (total == 0) return;
     const int64_t blocks = min(int64_t(gridDim.x), share(total + f.min_units - 1, 1, f.min_units));
     if (blockIdx.x >= blocks) return;
     int64_t at = share(total, blockIdx.x, blocks);
     const int64_t end = share(total, blockIdx.x + 1, blocks), start = at;
-    int s = 0;
     int64_t seq_at = 0;  // line position of sequence s
-    for (int s0 = 0; s0 < a.batch.seqs; s0 += 32) {
-        int64_t u = mine;
-        if (a.batch.seqs > 32) {
-            u = 0;
-            if (s0 + lane < a.batch.seqs) {
-                const SeqWork w = seq_work<UK, RT>(a, s0 + lane, f.most_rows);
-                u = int64_t(w.span()) * w.tiles * pl.heads;
-            }
-        }
-        int64_t run = u;
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += y;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, seq_at + run > at);
-        if (past) {
-            const int who = __ffs(past) - 1;
-            s = s0 + who;
-            seq_at += __shfl_sync(0xffffffffu, run - u, who);
-            break;
-        }
-        seq_at += __shfl_sync(0xffffffffu, run, 31);
+    int run = 0;
+    if (runs > 1) {
+        for (; run + 1 < runs && seq_at + run_sum[run] <= at; ++run) seq_at += run_sum[run];
+        mine = span_of(run * 32 + lane);
     }
+    int64_t upto = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, seq_at + upto > at);
+    const int who = past ? __ffs(past) - 1 : 0;
+    int s = run * 32 + who;
+    seq_at += __shfl_sync(0xffffffffu, upto - mine, who);
 
     while (at < end && s < a.batch.seqs) {
         const SeqWork w = seq_work<UK, RT>(a, s, f.most_rows);

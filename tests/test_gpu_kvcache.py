@@ -326,6 +326,17 @@ def test_attend_single_tokens(cuda, dtype, D, P):
         check_attend(cuda, [1] * len(lengths), lengths, H, G, D, P, dtype, seed=D + P + G, with_starts=False)
 
 
+@pytest.mark.parametrize("n", [31, 32, 33, 64, 65, 200, 500])
+def test_attend_many_sequences(cuda, n):
+    """Batches over several runs of 32 sequences, idle slots and rowless ones among them."""
+    rng = np.random.default_rng(n)
+    lengths = rng.integers(0, 80, n).tolist()
+    lengths[n // 2] = 1500
+    check_attend(cuda, [1] * n, lengths, 2, 4, 64, 16, seed=n, with_starts=False)
+    new = [min(int(k), x) for k, x in zip(rng.integers(0, 6, n), lengths)]
+    check_attend(cuda, new, lengths, 1, 3, 128, 32, "bf16", seed=n)
+
+
 @pytest.mark.parametrize("H,G", [(1, 1), (8, 1), (2, 3), (1, 7), (3, 5), (1, 16), (2, 12), (1, 33), (1, 64)])
 def test_attend_head_groups(cuda, H, G):
     check_attend(cuda, [1] * 5, [700, 1, 0, 64, 129], H, G, 128, 64, seed=G, with_starts=False, strided=True)
