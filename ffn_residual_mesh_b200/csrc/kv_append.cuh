@@ -11,7 +11,7 @@
 // in f32 before they are quantised.
 //
 // Bound by issue slots (rotation, two looks at a value, the quotient) and by the chain of dependent loads
-// before the values: 11.5k tokens of 8 kv heads x 128 with 32 heads of q, bf16: 66 us (3.6 TB/s);
+// before the values: 11.5k tokens of 8 kv heads x 128 with 32 heads of q, bf16: 65 us (3.7 TB/s);
 // 64 single tokens: 8.2 us. Reading them back in f32: 28 us (4.3 TB/s).
 #pragma once
 
