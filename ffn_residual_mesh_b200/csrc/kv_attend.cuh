@@ -6,11 +6,20 @@
 //   O = sum p_j vq_j,  out = O / l
 // so the value scale costs nothing per element and the weights of the codes stay in (0, 1]. A
 // row that sees no key gives zeros and lse = -inf.
+//
+// The logarithm and 1 / sv need sv well inside f32. A block with sv below kLeastScale holds values of
+// zero: it takes part with codes of zero under kZeroScale instead, so its keys keep their weight in l.
+// (kZeroScale is near the quantiser's floor of 1e-12, so such a block moves neither the maximum nor
+// the other blocks' p; with p = 2^-126 the smallest kept, l has weights down to 2^-86 against value scales of 1.)
 #pragma once
 
 #include "kv_common.cuh"
 
 namespace ffnrm::kv {
+
+constexpr float kLeastScale = 0x1p-64f, kZeroScale = 0x1p-40f;
+// Whether a block's values count as zero (a NaN or negative scale does not).
+__device__ __forceinline__ bool zero_block(float sv) { return fabsf(sv) < kLeastScale; }
 
 struct AttendArgs {
     Pool pool;

@@ -435,8 +435,19 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             const int64_t ph = int64_t(pg) * pl.heads + h;
             sc = make_float2(pl.k_scale[ph], pl.v_scale[ph]);
         };
-        auto fill = [&](bool v, int j, const uint4 (&r)[GROUPS * KB]) {  // wait for the stage, convert, hand over
+        auto fill = [&](bool v, int j, uint4 (&r)[GROUPS * KB]) {  // wait for the stage, convert, hand over
             const int st = j & 1;
+            if (v) {
+                const bool zero = zero_block(sc.y);
+                const unsigned runs = __ballot_sync(0xffffffffu, zero && lane < RUNS);
+#pragma unroll
+                for (int i = 0; i < RUNS; ++i)
+                    if (runs >> i & 1) {
+#pragma unroll
+                        for (int k = 0; k < 2 * KB; ++k) r[i * 2 * KB + k] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                if (zero) sc.y = kZeroScale;
+            }
             if (j >= 2 && !__all_sync(0xffffffffu, wait_phase((v ? v_empty : k_empty) + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty))) return false;
             // a NaN value scale reaches the rows that see it through its logarithm
             if (v && lane < RUNS)

@@ -346,7 +346,8 @@ int ffnrm_kv_read(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtyp
  * j <= position (causal, else all) and j > position - window (window > 0). f32 softmax
  * statistics. lse (optional, f32 [rows][q_heads]): natural log of the sum of exponentials. A
  * row that sees no key gives zeros and -inf; so do rows of idle slots and past starts[seqs].
- * A row that sees a token of a page whose scale is NaN is NaN (lse too). Pages that no row
+ * A row that sees a token of a page whose scale is NaN is NaN (lse too). A value scale of
+ * zero (or below 2^-64) makes values of zero whose keys keep their weight. Pages that no row
  * sees (before every window) are not looked up: their table entries may be -1. */
 int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, const ffnrm_rows *q,
                     const ffnrm_rows *out, float *lse, int q_heads, float scale, int causal, int window, void *stream);
