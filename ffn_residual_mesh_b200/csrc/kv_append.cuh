@@ -7,8 +7,8 @@
 // earlier codes become rint(q * (s_old / s)) and new ones rint(x / s) in [-127, 127], with IEEE
 // division, round-half-even and the 1e-12 floor of the groupwise activation quantiser
 // (scripts/benchmark_exact_radix_split_pipeline.py:39-47). A NaN or infinity among the new
-// values makes the scale NaN, so it reaches every row that reads the page. Keys are rotated
-// in f32 before they are quantised.
+// values makes the scale NaN, so it reaches every row that reads the page; so does an s_old that is
+// no scale (negative, infinite or NaN). Keys are rotated in f32 before they are quantised.
 //
 // Bound by issue slots (rotation, two looks at a value, the quotient) and by the chain of dependent loads
 // before the values: 11.5k tokens of 8 kv heads x 128 with 32 heads of q, bf16: 65 us (3.7 TB/s);
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) bits = max(bits, part[i]);
-    const bool bad = bits >= 0x7f800000u || before != before;
+    const bool bad = bits >= 0x7f800000u || sound_scale(before) != before;
     const float fresh = bad ? __int_as_float(0x7fffffff) : fmaxf(fmaxf(before, __fdiv_rn(__uint_as_float(bits), 127.f)), 1e-12f);
     if (threadIdx.x == 0) *scale = fresh;
     if (!bad && old && fresh != before) {

@@ -398,8 +398,18 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT, W>()) attend_few_ker
             if (next) load_k(u + 1, this_page);
             // z = y log2(e) + log2(sv); sc[n][i + 2 k]: key + g + 8 k, row 2t + i. A NaN value scale reaches the
             // rows that see it through its logarithm; it must not meet the others' p = 0.
-            const bool zero = zero_block(vs);
-            const float sv = zero ? kZeroScale : vs, vlog = lg2(sv), vinv = sv == sv ? __fdividef(1.f, sv) : 0.f;
+            // (One test for all unusual scales, which the page's whole warp takes alike.)
+            if (__float_as_uint(ks) >= 0x7f800000u || !(vs >= kLeastScale)) {
+                ks = sound_scale(ks);
+                if (zero_block(vs)) {
+                    vs = kZeroScale;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int c = 0; c < VB / 4; ++c) xv[r][c] = 0;
+                }
+            }
+            const float vlog = lg2(vs), vinv = vs == vs ? __fdividef(1.f, vs) : 0.f;
             const bool whole = key + 16 <= all_hi && key >= all_lo;
             bool raise = false;
 #pragma unroll
@@ -459,12 +469,6 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT, W>()) attend_few_ker
                 pb[n][1] = transpose8x8(pack_f16x2(p[2], p[3]));
             }
             // O^T += V^T P^T: channels (thread g: 16 g + ..) x rows, over the 16 keys
-            if (zero) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < VB / 4; ++c) xv[r][c] = 0;
-            }
 #pragma unroll
             for (int c = 0; c < VB / 4; ++c) {  // 4 channels each
                 const uint32_t lo01 = __byte_perm(xv[0][c], xv[1][c], 0x5140) ^ 0x80808080u, lo23 = __byte_perm(xv[0][c], xv[1][c], 0x7362) ^ 0x80808080u;

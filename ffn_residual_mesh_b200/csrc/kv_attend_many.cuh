@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                 if (lane == i) pg = page[i];
             if (pg < 0 || pg >= pl.pages) return;
             const int64_t ph = int64_t(pg) * pl.heads + h;
-            sc = make_float2(pl.k_scale[ph], pl.v_scale[ph]);
+            sc = make_float2(sound_scale(pl.k_scale[ph]), sound_scale(pl.v_scale[ph]));
         };
         auto fill = [&](bool v, int j, uint4 (&r)[GROUPS * KB]) {  // wait for the stage, convert, hand over
             const int st = j & 1;

@@ -77,6 +77,11 @@ __device__ __forceinline__ int seq_of_row(const int32_t *starts, int seqs, int r
     return lo;
 }
 
+// A stored scale as the kernels take it: finite and not negative, else NaN.
+__device__ __forceinline__ float sound_scale(float s) {
+    return s >= 0.f && s < __int_as_float(0x7f800000) ? s : __int_as_float(0x7fffffff);
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>

@@ -300,7 +300,8 @@ int ffnrm_rotary(const ffnrm_rows *x, const ffnrm_rows *y, int dtype, int tokens
 
 /* A cache of K and V as int8 codes in pages, with one f32 scale for each page and head:
  *   codes [n_layers][n_pages][kv_heads][page_tokens][head_dim], scales [n_layers][n_pages][kv_heads],
- *   value = code * scale.
+ *   value = code * scale. Scales are finite and not negative; NaN marks a block that took a non-finite
+ *   value, and append and attend take any other scale as that.
  * The four pools are the caller's device memory (codes 16-byte aligned), borrowed for the
  * handle's life. The handle owns a workspace: its calls must not overlap on the GPU (one
  * stream, or ordered by events), like a context's. All calls are asynchronous and

@@ -51,3 +51,38 @@ def test_value_scales_far_apart(cuda):
                 cache.v_scale[0, row[i]] = s
     check_attend(cuda, [1, 60], [300, 300], 2, 4, 128, 32, seed=8, tamper=uneven)
     check_attend(cuda, [280], [400], 2, 4, 128, 32, "bf16", seed=8, tamper=uneven)
+
+
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("value", [-0.02, -math.inf, math.inf])
+def test_scales_of_no_use_count_as_nan(cuda, which, value):
+    """A scale is finite and not negative; any other marks its block as a NaN does, in both kernels."""
+    import torch
+    tables, lengths = ints([[0, 1, 2, 3, 4, 5], [6, 7, 8, 9, 10, 11]], cuda), ints([300, 384], cuda)
+    for new in ([1, 1], [250, 130]):
+        got = []
+        for bad in (value, math.nan):
+            cache = make_cache(cuda, 12, 2, 128, 64, seed=3)
+            getattr(cache, which)[0, 1, 1] = bad  # tokens 64..127 of sequence 0, kv head 1
+            q = torch.randn(sum(new), 8, 128, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).half()
+            lse = torch.empty(sum(new), 8, device=cuda)
+            got.append((cache.attend(0, q, tables, lengths, starts=ints(row_starts(new), cuda), lse=lse), lse))
+            cache.check()
+        (out, lse), (want, want_lse) = got
+        assert torch.isnan(out[:new[0], 4:].float()).any() and not torch.isnan(out[:, :4]).any() and not torch.isnan(out[new[0]:]).any()
+        assert torch.equal(torch.nan_to_num(out, 9.0), torch.nan_to_num(want, 9.0))
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(torch.isnan(lse), torch.isnan(want_lse))
+
+
+@pytest.mark.parametrize("value", [-0.02, math.inf])
+def test_append_to_a_block_of_no_use_marks_it(cuda, value):
+    import torch
+    cache = make_cache(cuda, 3, 2, 64, 16)
+    cache.k_scale[0, 1, 0] = value
+    cache.v_scale[0, 1, 1] = value
+    x = torch.randn(1, 2, 64, device=cuda)
+    cache.append(0, x, x, ints([[0, 1]], cuda), ints([20], cuda))
+    cache.check()
+    assert torch.isnan(cache.k_scale[0, 1]).tolist() == [True, False]
+    assert torch.isnan(cache.v_scale[0, 1]).tolist() == [False, True]
