@@ -259,10 +259,8 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT, W>()) attend_few_ker
         const int all_lo = a.window > 0 ? max(0, pos0 + token_hi - a.window + 1) : 0;
 
         auto key_of = [&](int u) { return (w.unit0 + u) * UK + warp * 16; };
-        auto page_of = [&](int u) {
-            const int key = key_of(u);
-            return u < u1 && key < any_hi && key + 16 > any_lo ? table[key >> pl.page_shift] : -2;
-        };
+        auto needed = [&](int u) { return u < u1 && key_of(u) < any_hi && key_of(u) + 16 > any_lo; };
+        auto page_of = [&](int u) { return needed(u) ? table[key_of(u) >> pl.page_shift] : -1; };
         const int page = page_of(u0);
         int next_page = page_of(u0 + 1);  // on their way while the queries are read
 
@@ -328,9 +326,9 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT, W>()) attend_few_ker
         // 2t + 9. Each half is loaded again as soon as its product has used it.
         uint32_t xk[KV][2][4], xv[4][VB / 4];
         float ks = 0.f, vs = 1.f;
-        auto valid = [&](int page) {
+        auto valid = [&](int u, int page) {  // keys without a page are left out
             const bool have = unsigned(page) < unsigned(pl.pages);
-            if (!have && page != -2 && lane == 0) atomicOr(a.status, kStatusPage);
+            if (!have && needed(u) && lane == 0) atomicOr(a.status, kStatusPage);
             return have;
         };
         auto load_k = [&](int u, int page) {
@@ -364,13 +362,13 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT, W>()) attend_few_ker
             ks = pl.k_scale[ph];
             vs = pl.v_scale[ph];
         };
-        bool have = valid(page);
+        bool have = valid(u0, page);
         if (have) {
             load_k(u0, page);
             load_v(u0, page);
         }
         for (int u = u0; u < u1; ++u) {
-            const bool next = valid(next_page);
+            const bool next = valid(u + 1, next_page);
             const int key = key_of(u), this_page = next_page;
             next_page = page_of(u + 2);
             if (!have) {

@@ -382,20 +382,18 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
         const int32_t *table = a.batch.tables + int64_t(s) * a.batch.width;
         uint4 kr[GROUPS * KB];
         // lane: key lane / 4 of a group of eight, 16 channels lane % 4 of a block of 64
+        auto key_of = [&](int j, int i) { return (j0 + j) * BN + w * KEYS + i * 16; };
+        auto needed = [&](int j, int i) { return j < steps && key_of(j, i) < any_hi && key_of(j, i) + 16 > any_lo; };
         auto pages_of = [&](int j, int (&page)[RUNS]) {
 #pragma unroll
-            for (int i = 0; i < RUNS; ++i) {
-                const int key = (j0 + j) * BN + w * KEYS + i * 16;
-                page[i] = -2;
-                if (j < steps && key < any_hi && key + 16 > any_lo) page[i] = table[key >> pl.page_shift];
-            }
+            for (int i = 0; i < RUNS; ++i) page[i] = needed(j, i) ? table[key_of(j, i) >> pl.page_shift] : -1;
         };
         auto load = [&](int j, const int (&page)[RUNS], const int8_t *codes, uint4 (&r)[GROUPS * KB]) {
 #pragma unroll
             for (int i = 0; i < RUNS; ++i) {
-                const bool have = page[i] >= 0 && page[i] < pl.pages;
-                if (!have && page[i] != -2 && lane == 0) atomicOr(a.status, kStatusPage);
-                const int key = (j0 + j) * BN + w * KEYS + i * 16;
+                const bool have = unsigned(page[i]) < unsigned(pl.pages);
+                if (!have && lane == 0 && needed(j, i)) atomicOr(a.status, kStatusPage);
+                const int key = key_of(j, i);
                 const int64_t at = ((int64_t(have ? page[i] : 0) * pl.heads + h) * pl.page_tokens + (key & (pl.page_tokens - 1))) * D;
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
@@ -422,16 +420,18 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                         make_uint4(codes_f16x2<0>(u[2]), codes_f16x2<1>(u[2]), codes_f16x2<0>(u[3]), codes_f16x2<1>(u[3]));
                 }
         };
-        // the scales of run `lane` of a tile: loaded a tile ahead, as the page ids are two ahead
-        float2 sc = make_float2(0.f, 1.f);
+        // the scales of run `lane` of a tile: loaded a tile ahead, as the page ids are two ahead. Keys without a page
+        // (whose codes are zeros) weigh nothing: log2 sv = -inf and 1 / sv = 0
+        constexpr float kNoPage = -1.f;
+        float2 sc = make_float2(0.f, kNoPage);
         auto load_scales = [&](const int (&page)[RUNS]) {
-            sc = make_float2(0.f, 1.f);
+            sc = make_float2(0.f, kNoPage);
             if (lane >= RUNS) return;
             int pg = page[0];
 #pragma unroll
             for (int i = 1; i < RUNS; ++i)
                 if (lane == i) pg = page[i];
-            if (pg < 0 || pg >= pl.pages) return;
+            if (unsigned(pg) >= unsigned(pl.pages)) return;
             const int64_t ph = int64_t(pg) * pl.heads + h;
             sc = make_float2(sound_scale(pl.k_scale[ph]), sound_scale(pl.v_scale[ph]));
         };
@@ -451,7 +451,8 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             if (j >= 2 && !__all_sync(0xffffffffu, wait_phase((v ? v_empty : k_empty) + st, ((j >> 1) - 1) & 1, err, kErrWaitEmpty))) return false;
             // a NaN value scale reaches the rows that see it through its logarithm
             if (v && lane < RUNS)
-                sm_scale[st * C::CHUNKS + w * RUNS + lane] = make_float4(sc.x, lg2(sc.y), sc.y == sc.y ? __fdividef(1.f, sc.y) : 0.f, 0.f);
+                sm_scale[st * C::CHUNKS + w * RUNS + lane] =
+                    make_float4(sc.x, sc.y == kNoPage ? ninf : lg2(sc.y), sc.y > 0.f ? __fdividef(1.f, sc.y) : 0.f, 0.f);
             store((v ? sm_v : sm_k) + st * C::KV_BYTES, r);
             fence_proxy_async_smem();
             __syncwarp();

@@ -306,7 +306,8 @@ int ffnrm_rotary(const ffnrm_rows *x, const ffnrm_rows *y, int dtype, int tokens
  * handle's life. The handle owns a workspace: its calls must not overlap on the GPU (one
  * stream, or ordered by events), like a context's. All calls are asynchronous and
  * capturable. Data on the device that cannot be used (a page id outside the pool, a length
- * that does not fit) is skipped and recorded; ffnrm_kv_check reports it. */
+ * that does not fit) is skipped and recorded; ffnrm_kv_check reports it. (In attention the keys of
+ * such a page are left out of the softmax.) */
 typedef struct ffnrm_kv ffnrm_kv;
 typedef struct {
     int32_t n_layers;

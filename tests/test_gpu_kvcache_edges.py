@@ -86,3 +86,41 @@ def test_append_to_a_block_of_no_use_marks_it(cuda, value):
     cache.check()
     assert torch.isnan(cache.k_scale[0, 1]).tolist() == [True, False]
     assert torch.isnan(cache.v_scale[0, 1]).tolist() == [False, True]
+
+# ---------------------------------------------------------------------------------- tables
+@pytest.mark.parametrize("entry", [-1, -2, -3, -2 ** 31, 12, 2 ** 31 - 1])
+@pytest.mark.parametrize("new,G", [([1, 1], 4), ([3, 2], 4), ([90, 1], 4), ([130, 150], 8), ([180], 4)])
+def test_table_entries_that_name_no_page_are_skipped(cuda, entry, new, G):
+    """Whatever the entry, in either kernel: recorded, its keys left out, the others weighed as ever."""
+    import torch
+    import kv_reference as ref
+    H, D, P = 2, 128, 32
+    cache = make_cache(cuda, 12, H, D, P, seed=4)
+    rows, lengths = [[3, 7, 0, 11, 5, 1, 9], [2, 4, 6, 8, 10, 3, 7]][:len(new)], [220, 224][:len(new)]
+    q = torch.randn(sum(new), H * G, D, device=cuda, generator=torch.Generator(device=cuda).manual_seed(2)).half()
+    starts = row_starts(new)
+    broken = [list(r) for r in rows]
+    broken[0][0] = entry  # before every new token: the others see what the sequence without that page has
+    lse = torch.empty(sum(new), H * G, device=cuda)
+    out = cache.attend(0, q, ints(broken, cuda), ints(lengths, cuda), starts=ints(starts, cuda), lse=lse)
+    with pytest.raises(RuntimeError, match="page id"):
+        cache.check()
+    cache.check()
+    less, short = [r[1:] if i == 0 else r for i, r in enumerate(rows)], [lengths[0] - P] + lengths[1:]
+    want, mag, want_lse = ref.attend(q, cache.k_codes[0], cache.k_scale[0], cache.v_codes[0], cache.v_scale[0], less, short, starts)
+    if new[0] > short[0]:
+        raise AssertionError("the page must lie before the new tokens")
+    assert ((out.double() - want).abs() <= 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -13) * mag + 1e-6).all()
+    assert ((lse.double() - want_lse).abs() <= 2e-5 * want_lse.abs().clamp(min=1)).all()
+
+
+def test_a_table_of_no_pages_gives_zeros(cuda):
+    import torch
+    cache = make_cache(cuda, 4, 2, 128, 32)
+    for n in (1, 200):
+        q = torch.randn(n, 8, 128, device=cuda).half()
+        lse = torch.zeros(n, 8, device=cuda)
+        out = cache.attend(0, q, ints([[-2] * 8], cuda), ints([250], cuda), starts=ints([0, n], cuda), lse=lse)
+        with pytest.raises(RuntimeError, match="page id"):
+            cache.check()
+        assert (out == 0).all() and (lse == -math.inf).all()
