@@ -14,10 +14,10 @@
 // thread execute in order, so S of the next key tile may be written over P right behind the product
 // that reads it.
 //
-// Per 128 keys and 256 rows the products need 2048 cycles and the exponentials left to the MUFU 1536; the
-// loop takes 4300, the chain S - softmax - P - products with its hand-overs (116 cycles each) being
-// longer than either. Measured: 8192-token prompt, 32/8 heads x 128, causal: 596-620 us, 890-920
-// TFLOP/s (55% of the measured GEMM burst); 4096 tokens at head dim 256: 347 us.
+// Per 128 keys and 256 rows the products need 2048 cycles and the exponentials left to the MUFU 1792; the
+// loop takes some 4200, the chain S - softmax - P - products with its hand-overs (116 cycles each) being
+// longer than either. Measured: 8192-token prompt, 32/8 heads x 128, causal: 580-591 us, 930-948
+// TFLOP/s (57% of the measured GEMM burst); 4096 tokens at head dim 256: 350-357 us.
 #pragma once
 
 #include <type_traits>
@@ -312,8 +312,10 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                 m = to;
             }
             const float off = m == ninf ? 0.f : kFewOffset - m;
-            // two of every eight pairs take the polynomial, so that the MUFU (16 a clock for the SM, as
-            // long as both products of a tile) does not hold up the tensor cores; masked tiles need 2^-inf = 0
+            // One of eight pairs takes the polynomial, which relieves the MUFU (16 a clock for the SM, as long
+            // as both products of a tile). None / one / two / three of eight, in turns on one GPU, us: 8192-token prompt
+            // 617 / 591 / 611 / 618, three chunks of up to 2048 tokens 656 / 614 / 635 / 646, prompt of 1759 49.5 / 47.2 /
+            // 48.8 / 49.2, head dim 64 524 / 512 / 523 / 505, head dim 256 351 / 357 / 361 / 360. Masked tiles need 2^-inf = 0.
             auto weights = [&](auto polynomial) {
 #pragma unroll
                 for (int c = 0; c < BN; c += 32) {
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
                         for (int i = 0; i < 16; i += 2) {
                             float2 z = make_float2(__uint_as_float(x[c + half * 16 + i]), __uint_as_float(x[c + half * 16 + i + 1]));
                             z = ffma2(z, make_float2(f0, f0), make_float2(f1, f1));
-                            const float2 e = decltype(polynomial)::value && (i & 7) == 6 ? ex2_poly(z) : make_float2(ex2(z.x), ex2(z.y));
+                            const float2 e = decltype(polynomial)::value && i == 14 ? ex2_poly(z) : make_float2(ex2(z.x), ex2(z.y));
                             sum = i == 0 ? e : fadd2(sum, e);
                             p[half * 8 + i / 2] = pack_f16x2(e.x, e.y);
                         }
