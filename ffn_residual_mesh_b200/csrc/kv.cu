@@ -52,6 +52,11 @@ struct DeviceGuard {
 };
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+// Whether two ranges of memory share a byte.
+bool share_bytes(const void *a, size_t na, const void *b, size_t nb) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return na && nb && x < y + nb && y < x + na;
+}
 size_t type_size(int dtype) { return dtype == FFNRM_F32 ? 4 : 2; }
 
 // Whether a row block can be read in 16-byte accesses.
@@ -229,9 +234,9 @@ int device_setup(int device, const DeviceSetup *&out) {
             }
     KV_CUDA(prepare_many<__half>());
     KV_CUDA(prepare_many<__nv_bfloat16>());
-    // a bit for each of up to 2^20 pages, and 16 bytes for each of up to 4096 sequences
-    KV_CUDA(cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16));
-    KV_CUDA(cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 << 16));
+    // a bit for each of up to 2^20 pages, and 20 or 4 bytes for each of up to 4096 sequences
+    KV_CUDA(cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (1 << 17) + 20 * 4096));
+    KV_CUDA(cudaFuncSetAttribute(compact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (1 << 17) + 4 * 4096));
     d.done = true;
     return FFNRM_OK;
 }
@@ -518,12 +523,16 @@ int ffnrm_kv_fork(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, i
     if (!info || (children && (!parents || !extra || !out_lengths || (out_width && !out_tables))) ||
         (seqs && (!lengths || (table_width && !tables))))
         return fail(FFNRM_ERR_ARG, "null device pointer");
-    if (out_tables && out_tables == tables) return fail(FFNRM_ERR_ARG, "out_tables must not be the input tables");
+    const size_t table_bytes = size_t(seqs) * table_width * 4, out_bytes = size_t(children) * out_width * 4, length_bytes = size_t(children) * 4;
+    if (share_bytes(out_tables, out_bytes, tables, table_bytes)) return fail(FFNRM_ERR_ARG, "out_tables must not lie on the input tables");
+    if (share_bytes(out_tables, out_bytes, out_lengths, length_bytes) || share_bytes(info, 16, out_tables, out_bytes) ||
+        share_bytes(info, 16, out_lengths, length_bytes))
+        return fail(FFNRM_ERR_ARG, "out_tables, out_lengths and info must not lie on one another");
     DeviceGuard guard(kv->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const PageArgs a{tables, lengths, parents, extra, out_tables, out_lengths, info, kv->src, kv->dst, kv->count, kv->owner,
                      kv->list, seqs, table_width, children, out_width, kv->cfg.n_pages, kv->page_shift, kv->status};
-    fork_kernel<<<1, kPageThreads, size_t(kv->cfg.n_pages + 31) / 32 * 4 + size_t(children) * 16, st>>>(a);
+    fork_kernel<<<1, kPageThreads, size_t(kv->cfg.n_pages + 31) / 32 * 4 + size_t(children) * 20, st>>>(a);
     KV_CUDA(cudaGetLastError());
     if (children == 0) return FFNRM_OK;
     return launch_moves(kv, kv->src, kv->dst, kv->count, std::min(children, kv->cfg.n_pages), st);
@@ -537,6 +546,10 @@ int ffnrm_kv_compact(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths
         return fail(FFNRM_ERR_ARG, "table_width=%d must address at most 2^30 tokens", table_width);
     if (!info || (seqs && (!lengths || (table_width && (!tables || !out_tables)))))
         return fail(FFNRM_ERR_ARG, "null device pointer");
+    const size_t table_bytes = size_t(seqs) * table_width * 4;
+    if (out_tables != tables && share_bytes(out_tables, table_bytes, tables, table_bytes))
+        return fail(FFNRM_ERR_ARG, "out_tables must be the input tables or lie apart from them");
+    if (share_bytes(info, 16, out_tables, table_bytes)) return fail(FFNRM_ERR_ARG, "out_tables and info must not lie on one another");
     DeviceGuard guard(kv->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const PageArgs a{tables, lengths, nullptr, nullptr, out_tables, nullptr, info, kv->src, kv->dst, kv->count, kv->owner,

@@ -93,14 +93,16 @@ __device__ __forceinline__ void for_entries(int rows, int width, Get get, Put pu
         for_entries_of<int64_t>(total, width, get, put);
 }
 
-// One block. Shared memory: a bit per page, four integers per child. Bound by the latency of the
-// dependent loads (parent, length, table entry) and a dozen barriers.
+// One block. Shared memory: a bit per page, five integers per child. Bound by the latency of the
+// dependent loads (parent, length, table entry) and a dozen barriers. lengths, parents and extra are read before the
+// first barrier and out_lengths is written behind the last look at the tables, so it may lie on any of them.
 __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
     extern __shared__ uint32_t held[];
     __shared__ int flags;
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int words = (a.pages + 31) / 32, P = 1 << a.page_shift, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int *full = reinterpret_cast<int *>(held + words), *open = full + a.children, *need = open + a.children, *from = need + a.children;
+    int *full = reinterpret_cast<int *>(held + words), *open = full + a.children, *need = open + a.children, *from = need + a.children,
+        *grown = from + a.children;
     for (int i = tid; i < words; i += kPageThreads) held[i] = 0;
     if (tid == 0) flags = 0;
     __syncthreads();
@@ -139,7 +141,7 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
         full[c] = nf;
         open[c] = op;
         need[c] = ((length + grow + P - 1) >> a.page_shift) - nf;
-        a.out_lengths[c] = length + grow;
+        grown[c] = length + grow;
     }
     block_or(bad, &flags);
     // shared pages: a warp per child
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
         need[c] = offset;
         count[c] = n;
         offset += n;
-        if (refuse) a.out_lengths[c] = 0;
+        a.out_lengths[c] = refuse ? 0 : grown[c];
     }
     if (tid == 0) {
         a.info[kInfoUsed] = a.pages - free_total + (refuse ? 0 : want_total);

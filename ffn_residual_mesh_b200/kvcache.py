@@ -214,7 +214,9 @@ class PagedKvCache:
         """The next step's batch: child i continues sequence ``parents[i]`` (-1: an empty one)
         with room for ``extra[i]`` new tokens. A sequence named by several children is
         shared (its open last page is copied), one named by none is freed. Returns (tables,
-        lengths, info); info int32 [4] holds the pages held, free, copied and short."""
+        lengths, info); info int32 [4] holds the pages held, free, copied and short. ``out_lengths``
+        may be ``lengths`` (a fork that is short of pages leaves zeros there), ``out_tables`` lies apart
+        from ``tables``."""
         return self._calls.fork(self._geo, tables, lengths, parents, extra, out_tables, out_lengths, info, stream)
 
     def compact(self, tables, lengths, out_tables=None, info=None, stream=None):

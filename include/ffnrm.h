@@ -359,12 +359,12 @@ int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
  * tokens (parents[i] = -1: an empty one; a sequence that no child names is freed). Full
  * pages are shared; an open last page is kept by one child and copied for the others, in
  * every layer; new pages are the lowest free ids in child order. out_tables
- * [children][out_width] (-1 past the end; not the input's memory), out_lengths [children];
- * info int32 [4]: pages held, free, copied, and short. With too few free pages nothing is
- * copied, the outputs are empty sequences, info[3] says how many are missing and
- * ffnrm_kv_check reports FFNRM_ERR_NOMEM; the input tables stay valid.
- * compact: moves the held pages to the lowest ids, in every layer; out_tables (may be the
- * input) names the new places; info: pages held, free, moved, 0.
+ * [children][out_width] (-1 past the end; not on the input tables), out_lengths [children]
+ * (may lie on lengths, parents or extra); info int32 [4]: pages held, free, copied, and short. With too
+ * few free pages nothing is copied, the outputs are empty sequences, info[3] says how many are missing and
+ * ffnrm_kv_check reports FFNRM_ERR_NOMEM; inputs that no output lies on stay valid.
+ * compact: moves the held pages to the lowest ids, in every layer; out_tables (the
+ * input or apart from it) names the new places; info: pages held, free, moved, 0.
  * copy_pages: page src[i] to dst[i] for i < n, in every layer (device lists; a page named
  * as a destination is named once and is no source). */
 int ffnrm_kv_fork(ffnrm_kv *kv, const int32_t *tables, const int32_t *lengths, int seqs, int table_width,

@@ -124,3 +124,65 @@ def test_a_table_of_no_pages_gives_zeros(cuda):
         with pytest.raises(RuntimeError, match="page id"):
             cache.check()
         assert (out == 0).all() and (lse == -math.inf).all()
+
+
+# ---------------------------------------------------------------------------------- fork in place
+@pytest.mark.parametrize("n", [6, 33, 700, 2500])
+def test_fork_writes_lengths_in_place(cuda, n):
+    """out_lengths on the input lengths, parents in any order: the same as apart from them."""
+    import numpy as np
+    import torch
+    rng = np.random.default_rng(n)
+    P, width = 16, 5
+    lengths = rng.integers(0, 3 * P, n)
+    rows, at = [], 0
+    for x in lengths:
+        k = -(-int(x) // P)
+        rows.append([*range(at, at + k), *[-1] * (width - k)])
+        at += k
+    parents = rng.permutation(n)
+    parents[rng.integers(0, n, n // 5)] = int(parents[0])
+    extra = rng.integers(0, P, n)
+    cache = make_cache(cuda, at + 4 * n, 1, 64, P, max_seqs=n)
+    args = [ints(v, cuda) for v in (rows, lengths.tolist(), parents.tolist(), extra.tolist())]
+    tables, lens, info = cache.fork(*args)
+    cache.check()
+    assert lens.tolist() == (lengths[parents] + extra).tolist()
+    for place in (1, 2, 3):  # on the lengths, the parents, the room
+        own = [a.clone() for a in args]
+        got, out, got_info = cache.fork(*own, out_lengths=own[place])
+        cache.check()
+        assert out.data_ptr() == own[place].data_ptr()
+        assert torch.equal(got, tables) and torch.equal(out, lens) and torch.equal(got_info, info)
+    buffer = torch.cat([args[1], ints([0] * 8, cuda)])  # shifted by some
+    got, out, _ = cache.fork(args[0], buffer[:n], *args[2:], out_lengths=buffer[5:n + 5])
+    cache.check()
+    assert torch.equal(got, tables) and torch.equal(out, lens)
+
+
+def test_fork_short_of_pages_in_place(cuda):
+    """Nothing is forked: zeros where out_lengths lies, be it the input."""
+    cache = make_cache(cuda, 3, 1, 64, 16)
+    tables, lengths, extra = ints([[0, 1, 2, -1]], cuda), ints([40], cuda), ints([16], cuda)
+    for out in (None, lengths):
+        _, lens, info = cache.fork(tables, lengths, ints([0], cuda), extra, out_lengths=out)
+        with pytest.raises(MemoryError):
+            cache.check()
+        assert lens.tolist() == [0] and info.tolist() == [3, 0, 0, 1] and lengths.tolist() == [40 if out is None else 0]
+
+
+def test_page_tables_on_one_another_are_refused(cuda):
+    import torch
+    cache = make_cache(cuda, 40, 1, 64, 16)
+    buffer = torch.zeros(64, dtype=torch.int32, device=cuda)
+    n, p, e = ints([5, 20], cuda), ints([0, 1], cuda), ints([1, 1], cuda)
+    t = buffer[:6].view(2, 3)
+    for call in (lambda: cache.fork(t, n, p, e, out_tables=t), lambda: cache.fork(t, n, p, e, out_tables=buffer[5:11].view(2, 3)),
+                 lambda: cache.fork(t, n, p, e, out_tables=buffer[10:16].view(2, 3), out_lengths=buffer[15:17]),
+                 lambda: cache.fork(t, n, p, e, out_tables=buffer[10:16].view(2, 3), info=buffer[7:11]),
+                 lambda: cache.fork(t, n, p, e, out_lengths=buffer[20:22], info=buffer[21:25]),
+                 lambda: cache.compact(t, n, out_tables=buffer[3:9].view(2, 3)), lambda: cache.compact(t, n, info=buffer[5:9], out_tables=t)):
+        with pytest.raises(ValueError):
+            call()
+    cache.fork(t, n, p, e, out_tables=buffer[6:12].view(2, 3), out_lengths=buffer[12:14], info=buffer[14:18])  # side by side
+    cache.check()
