@@ -32,21 +32,22 @@ struct PageArgs {
 };
 
 // Exclusive scan of one value per thread over the block; `total` is the sum.
-__device__ __forceinline__ int block_scan(int v, int &total) {
-    __shared__ int sums[kPageThreads / 32];
+template <typename Int>
+__device__ __forceinline__ Int block_scan(Int v, Int &total) {
+    __shared__ Int sums[kPageThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    Int x = v;
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const Int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) sums[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        int y = sums[lane];
+        Int y = sums[lane];
         for (int o = 1; o < 32; o <<= 1) {
-            const int z = __shfl_up_sync(0xffffffffu, y, o);
+            const Int z = __shfl_up_sync(0xffffffffu, y, o);
             if (lane >= o) y += z;
         }
         sums[lane] = y;
@@ -184,7 +185,8 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
         const int n = a.pages - w * 32;
         return ~held[w] & (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
     };
-    int mine = 0, free_total, want = 0, want_total;
+    int mine = 0, free_total;
+    int64_t want = 0, want_total;  // 4096 children may ask for 2^26 pages each
     for (int w = w0; w < w1; ++w) mine += __popc(free_bits(w));
     int rank = block_scan(mine, free_total);
     const int cper = (a.children + kPageThreads - 1) / kPageThreads, c0 = tid * cper, c1 = min(a.children, c0 + cper);
@@ -193,9 +195,9 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
         want += need[c];
         copies += open[c] >= 0 && full[c] >= 0;
     }
-    int offset = block_scan(want, want_total);
+    int64_t offset = block_scan(want, want_total);
     int copy_at = block_scan(copies, copies_total);
-    const int shortage = max(0, want_total - free_total);
+    const int shortage = int(min(max(want_total - free_total, int64_t(0)), int64_t(0x7fffffff)));
     const bool refuse = shortage || bad;
     for (int w = w0; w < w1 && rank < want_total; ++w) {
         for (uint32_t b = free_bits(w); b; b &= b - 1) {
@@ -212,14 +214,14 @@ __global__ void __launch_bounds__(kPageThreads) fork_kernel(PageArgs a) {
             a.dst[copy_at] = a.list[offset];
             ++copy_at;
         }
-        need[c] = offset;
+        need[c] = refuse ? 0 : int(offset);
         count[c] = n;
         offset += n;
         a.out_lengths[c] = refuse ? 0 : grown[c];
     }
     if (tid == 0) {
-        a.info[kInfoUsed] = a.pages - free_total + (refuse ? 0 : want_total);
-        a.info[kInfoFree] = free_total - (refuse ? 0 : want_total);
+        a.info[kInfoUsed] = a.pages - free_total + (refuse ? 0 : int(want_total));
+        a.info[kInfoFree] = free_total - (refuse ? 0 : int(want_total));
         a.info[kInfoMoved] = refuse ? 0 : copies_total;
         a.info[kInfoShort] = shortage;
         *a.count = refuse ? 0 : copies_total;

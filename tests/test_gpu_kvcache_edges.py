@@ -186,3 +186,18 @@ def test_page_tables_on_one_another_are_refused(cuda):
             call()
     cache.fork(t, n, p, e, out_tables=buffer[6:12].view(2, 3), out_lengths=buffer[12:14], info=buffer[14:18])  # side by side
     cache.check()
+
+
+def test_fork_that_asks_for_more_than_2_to_the_31_pages(cuda):
+    """The children's wishes add up past 32 bits: short of pages, nothing changed."""
+    import torch
+    n, width = 2049, 1 << 20
+    cache = make_cache(cuda, 3, 1, 64, 16, max_seqs=n)
+    before = cache.k_codes.clone()
+    out = torch.empty(n, width, dtype=torch.int32, device=cuda)
+    tables, lens, info = cache.fork(ints([[0, 1]], cuda), ints([20], cuda), ints([0] + [-1] * (n - 1), cuda),
+                                    torch.full((n,), 16 * width - 32, dtype=torch.int32, device=cuda), out_tables=out)
+    with pytest.raises(MemoryError):
+        cache.check()
+    assert (lens == 0).all() and info.tolist() == [2, 1, 0, 2 ** 31 - 1]
+    assert (tables[:: 512] == -1).all() and torch.equal(cache.k_codes, before)
