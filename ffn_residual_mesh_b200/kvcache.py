@@ -86,7 +86,7 @@ class RotaryTable:
             # the (fractional) pair that makes `turns` turns within the original context
             at = [rotary_dim * math.log(original_positions / (turns * 2 * math.pi)) / (2 * math.log(base))
                   for turns in (beta_fast, beta_slow)]
-            low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary_dim // 2 - 1)
+            low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary_dim - 1)
             ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
             freq = freq * (1 - ramp) + freq / factor * ramp
             gain = 0.1 * math.log(factor) + 1.0

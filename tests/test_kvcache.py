@@ -101,3 +101,29 @@ def test_null_cache_and_rotary_arguments_are_refused():
                dict(y=N.Rows(64, 128, 64)), dict(x=N.Rows(65, 64, 64))):
         assert rotary(**kw) == N.ERR_ARG, kw
     assert rotary(tokens=0) == N.OK and rotary(heads=0) == N.OK
+
+
+@pytest.mark.parametrize("R,base,orig,factor", [(128, 1e4, 131072, 8.0), (128, 1e4, 8192, 4.0), (64, 1e4, 65536, 16.0), (32, 500.0, 1000000, 2.0),
+                                                (256, 1e6, 4096, 8.0), (16, 1e4, 300, 32.0)])
+def test_yarn_ramp_where_the_last_pair_lies_inside_it(R, base, orig, factor):
+    """Pairs of more than 32 turns stay and those below one turn are divided, whichever end of the head the ramp
+    reaches; between them the ramp is straight from floor to ceil of its fractional pairs, held to [0, R - 1]."""
+    t = table(R, 64, base=base, scaling="yarn", factor=factor, original_positions=orig)
+    angle = angles(t)[1]
+    low = max(math.floor(R * math.log(orig / (64 * math.pi)) / (2 * math.log(base))), 0)
+    high = min(math.ceil(R * math.log(orig / (2 * math.pi)) / (2 * math.log(base))), R - 1)
+    for i in range(R // 2):
+        f = base ** (-2 * i / R)
+        turns = orig * f / (2 * math.pi)
+        ramp = min(max((i - low) / (high - low), 0.0), 1.0)
+        assert (turns <= 32 or ramp == 0) and (turns >= 1 or ramp == 1)
+        p = np.arange(64) * (f * (1 - ramp) + f / factor * ramp)
+        off = (angle[:, i] - p + math.pi) % (2 * math.pi) - math.pi
+        assert np.abs(off).max() < 1e-5, (i, f, ramp)
+
+
+def test_yarn_last_pair_of_a_long_trained_context():
+    """2.4 turns in 131072 positions: 0.37 of its frequency, not an eighth."""
+    t = table(128, 8, base=1e4, scaling="yarn", factor=8.0, original_positions=131072)
+    got = angles(t)[1][1, 63] / 1e4 ** (-126 / 128)
+    assert abs(got - 0.37) < 0.01
