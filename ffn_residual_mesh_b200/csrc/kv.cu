@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <mutex>
 #include <new>
 
@@ -68,6 +69,61 @@ bool wide(const ffnrm_rows &r, int dtype) {
 int check_rows(const char *name, const ffnrm_rows *r, int dtype) {
     if (!r || !r->data) return fail(FFNRM_ERR_ARG, "%s: null rows", name);
     if (!aligned(r->data, type_size(dtype))) return fail(FFNRM_ERR_ARG, "%s: misaligned rows", name);
+    return FFNRM_OK;
+}
+
+// The least |e + a stride| over whole numbers |a| <= most is below dim.
+bool comes_near(int64_t e, int64_t stride, int64_t most, int64_t dim) {
+    if (stride == 0 || most <= 0) return std::abs(e) < dim;
+    const int64_t a = -e / stride;  // the nearest is one of its neighbours, or the end of the range
+    for (int64_t i = a - 1; i <= a + 1; ++i)
+        if (std::abs(e + std::clamp(i, -most, most) * stride) < dim) return true;
+    return false;
+}
+
+// Row blocks of `tokens` rows: x with hx heads and y with hy, rows of dim elements of one type.
+struct RowPair {
+    int64_t tokens, hx, hy, dim;
+    size_t size;
+};
+// First byte and end of a block.
+void extent(const ffnrm_rows &r, int64_t tokens, int64_t heads, const RowPair &p, uintptr_t &lo, uintptr_t &hi) {
+    const int64_t t = (tokens - 1) * r.token_stride, h = (heads - 1) * r.head_stride;
+    lo = reinterpret_cast<uintptr_t>(r.data) + (std::min<int64_t>(t, 0) + std::min<int64_t>(h, 0)) * int64_t(p.size);
+    hi = reinterpret_cast<uintptr_t>(r.data) + (std::max<int64_t>(t, 0) + std::max<int64_t>(h, 0) + p.dim) * int64_t(p.size);
+}
+bool same_rows(const ffnrm_rows &x, const ffnrm_rows &y, const RowPair &p) {
+    return x.data == y.data && p.hx == p.hy && (p.tokens == 1 || x.token_stride == y.token_stride) &&
+           (p.hx == 1 || x.head_stride == y.head_stride);
+}
+// Whether x and y share an element. Blocks that lie in one another's gaps (slices of packed rows) do not, which is
+// found where they have one token stride; with two different ones they count as sharing.
+bool rows_meet(const ffnrm_rows &x, const ffnrm_rows &y, const RowPair &p) {
+    uintptr_t x0, x1, y0, y1;
+    extent(x, p.tokens, p.hx, p, x0, x1);
+    extent(y, p.tokens, p.hy, p, y0, y1);
+    if (x0 >= y1 || y0 >= x1) return false;
+    if (p.tokens > 1 && x.token_stride != y.token_stride) return true;
+    const int64_t d = (reinterpret_cast<intptr_t>(y.data) - reinterpret_cast<intptr_t>(x.data)) / int64_t(p.size);
+    const bool alike = x.head_stride == y.head_stride;  // then only the difference of the heads counts
+    for (int64_t i = 0; i < p.hx; ++i)
+        for (int64_t j = 0; j < (alike && i ? 1 : p.hy); ++j)
+            if (comes_near(d + j * y.head_stride - i * x.head_stride, x.token_stride, p.tokens - 1, p.dim)) return true;
+    return false;
+}
+// Whether two rows of a block share an element.
+bool rows_fold(const ffnrm_rows &x, int64_t tokens, int64_t heads, int64_t dim) {
+    const int64_t st = x.token_stride, sh = x.head_stride;
+    if (sh >= dim && st >= (heads - 1) * sh + dim) return false;  // rows one behind another
+    if (tokens > 1 && std::abs(st) < dim) return true;
+    for (int64_t b = 1; b < heads; ++b)
+        if (comes_near(b * sh, st, tokens - 1, dim)) return true;
+    return false;
+}
+// Rows that a kernel writes: apart from one another, and the rows that it reads meanwhile or apart from them.
+int check_written(const char *name, const ffnrm_rows &y, const char *from, const ffnrm_rows &x, const RowPair &p) {
+    if (rows_fold(y, p.tokens, p.hy, p.dim)) return fail(FFNRM_ERR_ARG, "%s: rows lie on one another", name);
+    if (!same_rows(x, y, p) && rows_meet(x, y, p)) return fail(FFNRM_ERR_ARG, "%s must be %s itself or lie apart from it", name, from);
     return FFNRM_OK;
 }
 
@@ -314,9 +370,8 @@ int ffnrm_rotary(const ffnrm_rows *x, const ffnrm_rows *y, int dtype, int tokens
     if (rc) return rc;
     if (tokens == 0 || heads == 0) return FFNRM_OK;
     if ((rc = check_rows("x", x, dtype)) || (rc = check_rows("y", y, dtype))) return rc;
+    if ((rc = check_written("y", *y, "x", *x, RowPair{tokens, heads, heads, head_dim, type_size(dtype)}))) return rc;
     if (!positions || !aligned(positions, 4)) return fail(FFNRM_ERR_ARG, "null or misaligned positions");
-    if (x->data == y->data && (x->token_stride != y->token_stride || x->head_stride != y->head_stride))
-        return fail(FFNRM_ERR_ARG, "rotating in place needs equal strides");
     if (int64_t(tokens) * heads * head_dim / 256 > 0x7fffffff) return fail(FFNRM_ERR_ARG, "tokens=%d are too many for one call", tokens);
     const RotaryArgs a{x->data, y->data, positions, table, x->token_stride, x->head_stride, y->token_stride, y->head_stride,
                        tokens, heads, head_dim, rotary_dim, max_positions};
@@ -427,8 +482,10 @@ int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     if ((rc = check_rows("k", k, dtype)) || (rc = check_rows("v", v, dtype))) return rc;
     if (has_q) {
         if ((rc = check_rows("q_out", q_out, dtype)) || (rc = check_rows("q", q, dtype))) return rc;
-        if (q->data == q_out->data && (q->token_stride != q_out->token_stride || q->head_stride != q_out->head_stride))
-            return fail(FFNRM_ERR_ARG, "rotating in place needs equal strides");
+        const size_t size = type_size(dtype);
+        if ((rc = check_written("q_out", *q_out, "q", *q, RowPair{batch->rows, q_heads, q_heads, D, size}))) return rc;
+        const RowPair kv_pair{batch->rows, kv->cfg.kv_heads, q_heads, D, size};
+        if (rows_meet(*k, *q_out, kv_pair) || rows_meet(*v, *q_out, kv_pair)) return fail(FFNRM_ERR_ARG, "q_out must lie apart from k and v");
     }
     const bool inter = flags & FFNRM_ROTARY_INTERLEAVED;
     const int N = 16 / int(type_size(dtype));
@@ -497,6 +554,15 @@ int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     if (!wide(*q, dtype) || !wide(*out, dtype))
         return fail(FFNRM_ERR_ARG, "q and out rows must be 16-byte aligned");
     if (!aligned(lse, 4)) return fail(FFNRM_ERR_ARG, "lse must be 4-byte aligned");
+    const RowPair pair{batch->rows, q_heads, q_heads, kv->cfg.head_dim, type_size(dtype)};
+    if ((rc = check_written("out", *out, "q", *q, pair))) return rc;
+    if (lse)
+        for (const ffnrm_rows *r : {q, out}) {
+            uintptr_t lo, hi;
+            extent(*r, batch->rows, q_heads, pair, lo, hi);
+            if (share_bytes(lse, size_t(batch->rows) * q_heads * 4, reinterpret_cast<const void *>(lo), hi - lo))
+                return fail(FFNRM_ERR_ARG, "lse must lie apart from q and out");
+        }
     window = std::min(window, 1 << 30);  // no sequence is longer; keeps position - window in 32 bits
     const AttendArgs a{layer_pool(kv, layer), batch_view(batch), q->data, out->data, lse, q->token_stride, q->head_stride,
                        out->token_stride, out->head_stride, q_heads / kv->cfg.kv_heads, scale, causal, window, kv->status};

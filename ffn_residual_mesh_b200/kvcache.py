@@ -114,7 +114,7 @@ class RotaryTable:
 def rotary(x, positions, table: RotaryTable, out=None, inverse: bool = False, stream=None):
     """x [T, heads, dim] with its first ``rotary_dim`` channels rotated at ``positions`` (int32
     [T]); ``inverse`` applies the transposed rotation, the gradient of the forward one.
-    ``out`` may be x. A position outside the table gives NaN in the rotated channels."""
+    ``out`` is x or lies apart from it. A position outside the table gives NaN in the rotated channels."""
     return (_module or _bind()).rotary(x, positions, table.cos_sin, out, table.flags | (N.ROTARY_INVERSE if inverse else 0), stream)
 
 
@@ -187,14 +187,16 @@ class PagedKvCache:
                stream=None):
         """Quantise the step's new k and v [T, kv_heads, head_dim] into their pages. With
         ``rope`` the keys are rotated at their positions first, and with ``q`` [T, heads,
-        head_dim] the queries too; returns the rotated queries (``q_out``, which may be q)."""
+        head_dim] the queries too; returns the rotated queries (``q_out``, which is q or lies
+        apart from q, k and v)."""
         return self._calls.append(self._geo, layer, k, v, tables, lengths, starts, rope.cos_sin if rope else None,
                                   rope.flags if rope else 0, q, q_out, stream)
 
     def attend(self, layer: int, q, tables, lengths, starts=None, out=None, lse=None, scale: float | None = None,
                causal: bool = True, window: int = 0, stream=None):
         """Attention of the step's queries q [T, heads, head_dim] (float16 or bfloat16) over the
-        cache, the step's own tokens included. ``scale`` defaults to ``head_dim ** -0.5``;
+        cache, the step's own tokens included. q's and ``out``'s rows start on 16 bytes (views of packed
+        rows do where head_dim divides their offsets); ``out`` is q or lies apart from it. ``scale`` defaults to ``head_dim ** -0.5``;
         ``window`` > 0 lets a query see its last ``window`` positions only. ``lse`` (float32
         [T, heads]) receives the natural log of the sum of exponentials."""
         return self._calls.attend(self._geo, layer, q, tables, lengths, starts, out, lse,

@@ -291,7 +291,8 @@ typedef struct {
  * of `table` f32 [max_positions][rotary_dim] (rotary_dim/2 cosines, then the sines). Pair i
  * is channels (i, i + rotary_dim/2), or (2i, 2i + 1) with FFNRM_ROTARY_INTERLEAVED;
  * FFNRM_ROTARY_INVERSE applies the transposed rotation (the gradient). f32 arithmetic, one
- * rounding. y may be x. A position outside the table gives NaN in the rotated channels. */
+ * rounding. y is x or lies apart from it (slices of one packed row do; rows in one another's gaps need equal
+ * token strides). A position outside the table gives NaN in the rotated channels. */
 #define FFNRM_ROTARY_INTERLEAVED 1
 #define FFNRM_ROTARY_INVERSE 2
 int ffnrm_rotary(const ffnrm_rows *x, const ffnrm_rows *y, int dtype, int tokens, int heads, int head_dim,
@@ -334,7 +335,8 @@ int ffnrm_kv_destroy(ffnrm_kv *kv);
  * with s_old the scale where the page already holds earlier tokens; earlier codes become
  * rint(q * (s_old / s)), new ones rint(x / s). Non-finite values make the scale NaN. With
  * `table` the keys are rotated at their positions first, and with q, q_out as well the
- * queries [rows][q_heads][head_dim] (q_out may be q; rows of idle slots become zeros). */
+ * queries [rows][q_heads][head_dim] (q_out is q or lies apart from it, and apart from k and v; rows of
+ * idle slots become zeros). */
 int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, const ffnrm_rows *k,
                     const ffnrm_rows *v, const ffnrm_rows *q, const ffnrm_rows *q_out, int q_heads, const float *table,
                     int rotary_dim, int max_positions, int flags, void *stream);
@@ -350,7 +352,8 @@ int ffnrm_kv_read(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtyp
  * row that sees no key gives zeros and -inf; so do rows of idle slots and past starts[seqs].
  * A row that sees a token of a page whose scale is NaN is NaN (lse too). A value scale of
  * zero (or below 2^-64) makes values of zero whose keys keep their weight. Pages that no row
- * sees (before every window) are not looked up: their table entries may be -1. */
+ * sees (before every window) are not looked up: their table entries may be -1. q and out rows are 16-byte
+ * aligned (base and strides); out is q or lies apart from it. */
 int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, const ffnrm_rows *q,
                     const ffnrm_rows *out, float *lse, int q_heads, float scale, int causal, int window, void *stream);
 

@@ -201,3 +201,67 @@ def test_fork_that_asks_for_more_than_2_to_the_31_pages(cuda):
         cache.check()
     assert (lens == 0).all() and info.tolist() == [2, 1, 0, 2 ** 31 - 1]
     assert (tables[:: 512] == -1).all() and torch.equal(cache.k_codes, before)
+
+
+# ---------------------------------------------------------------------------------- memory that overlaps
+def test_overlapping_outputs_are_refused(cuda):
+    import torch
+    from ffn_residual_mesh_b200.kvcache import rotary
+    H, G, D, T = 2, 4, 64, 6
+    cache = make_cache(cuda, 8, H, D, 16)
+    tables, lengths, starts = ints([[0, 1], [2, 3]], cuda), ints([20, 9], cuda), ints([0, 4, 6], cuda)
+    table, pos = rope_table(64, D, cuda), ints([0, 1, 2, 3, 4, 5], cuda)
+    qkv = torch.randn(T + 1, H * G + 2 * H + 1, D, device=cuda).half()
+    q, k, v = qkv[:T, :H * G], qkv[:T, H * G:H * G + H], qkv[:T, H * G + H:H * G + 2 * H]
+    flat, args = qkv.flatten(), dict(starts=starts, rope=table, q=q)
+    before = [t.clone() for t in (qkv, cache.k_codes, cache.v_codes)]
+    for call in (lambda: rotary(q, pos, table, out=qkv[:T, 1:H * G + 1]), lambda: rotary(q, pos, table, out=qkv[1:, :H * G]),
+                 lambda: rotary(q, pos, table, out=flat[:T * H * G * D].view(T, H * G, D)),
+                 lambda: rotary(q, pos, table, out=torch.empty(999 * D, device=cuda).half().as_strided((T, H * G, D), (D, D, 1))),
+                 lambda: cache.append(0, k, v, tables, lengths, q_out=qkv[:T, 2:H * G + 2], **args),
+                 lambda: cache.append(0, k, v, tables, lengths, q_out=qkv[:T, H + 1:H * G + H + 1], **args),
+                 lambda: cache.append(0, k, qkv[:T, :H].clone(), tables, lengths, q_out=qkv[:T, 2 * H:H * G + 2 * H], **dict(args, q=q.clone())),
+                 lambda: cache.attend(0, q, tables, lengths, starts=starts, out=qkv[:T, 1:H * G + 1]),
+                 lambda: cache.attend(0, q, tables, lengths, starts=starts, out=qkv[1:, :H * G]),
+                 lambda: cache.attend(0, q, tables, lengths, starts=starts, lse=flat.view(torch.float32)[:T * H * G].view(T, H * G))):
+        with pytest.raises(ValueError):
+            call()
+    cache.check()
+    for a, b in zip(before, (qkv, cache.k_codes, cache.v_codes)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [5, 3], [150, 90]])
+def test_in_place_and_in_a_packed_row(cuda, new):
+    """q rotated and attended in place, and into another slice of its own packed row: as into memory apart."""
+    import torch
+    from ffn_residual_mesh_b200.kvcache import rotary
+    H, G, D = 2, 4, 128
+    T, lengths = sum(new), ints([200, 90], cuda)
+    tables, starts = ints([[*range(13)], [*range(13, 26)]], cuda), ints(row_starts(new), cuda)
+    table = rope_table(256, D, cuda)
+    packed = torch.randn(T, 2 * H * G + 2 * H, D, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).half()
+
+    def step(q, out, k, v):
+        cache = make_cache(cuda, 26, H, D, 16, seed=1)
+        got = cache.append(0, k, v, tables, lengths, starts=starts, rope=table, q=q, q_out=out)
+        rotated = got.clone()
+        seen = cache.attend(0, got, tables, lengths, starts=starts, out=out)
+        cache.check()
+        return rotated, seen
+
+    def parts(x):
+        return x[:, :H * G], x[:, H * G:2 * H * G], x[:, 2 * H * G:2 * H * G + H], x[:, 2 * H * G + H:]
+
+    q, _, k, v = parts(packed.clone())
+    want = step(q, torch.empty_like(q), k, v)
+    q, spare, k, v = parts(packed.clone())
+    got = step(q, spare, k, v)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(q, packed[:, :H * G])
+    q, _, k, v = parts(packed.clone())
+    got = step(q, q, k, v)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x = packed.clone()
+    pos = torch.arange(T, device=cuda).int()
+    rotary(x[:, :H], pos, table, out=x[:, H:2 * H])
+    assert torch.equal(x[:, H:2 * H], rotary(packed[:, :H], pos, table)) and torch.equal(x[:, 2 * H:], packed[:, 2 * H:])

@@ -127,3 +127,35 @@ def test_yarn_last_pair_of_a_long_trained_context():
     t = table(128, 8, base=1e4, scaling="yarn", factor=8.0, original_positions=131072)
     got = angles(t)[1][1, 63] / 1e4 ** (-126 / 128)
     assert abs(got - 0.37) < 0.01
+
+
+def test_overlapping_rows_are_refused():
+    """Written rows lie apart from one another, and on the rows that are read or apart from them: against the sets
+    of elements, over random layouts. (Null positions end each call before any launch.)"""
+    import random
+    from ffn_residual_mesh_b200 import _native as N
+    lib, rng, seen = N.lib(), random.Random(1), [0, 0, 0]
+
+    def elements(at, T, H, st, sh, dim):
+        return [at + t * st + h * sh + i for t in range(T) for h in range(H) for i in range(dim)]
+
+    for _ in range(6000):
+        T, H, dim = rng.randint(1, 4), rng.randint(1, 3), rng.choice([2, 4, 6])
+        sx = rng.choice([(H * dim, dim), (dim, T * dim), (2 * H * dim, dim), (3 * dim * H, 3 * dim), (dim + 1, 9), (rng.randint(0, 40), rng.randint(0, 12))])
+        sy = sx if rng.random() < 0.6 else (rng.randint(0, 40), rng.choice([dim, dim + 1, 2 * dim]))
+        d = rng.choice([0, dim, H * dim, rng.randint(-60, 60)])
+        x, y = elements(1000, T, H, *sx, dim), elements(1000 + d, T, H, *sy, dim)
+        size = 4
+        xr, yr = N.Rows(size * 1000, *sx), N.Rows(size * (1000 + d), *sy)
+        assert lib.ffnrm_rotary(ctypes.byref(xr), ctypes.byref(yr), N.F32, T, H, dim, None, 16, 2, 4, 0, None) == N.ERR_ARG
+        message = lib.ffnrm_last_error().decode()
+        if len(set(y)) < len(y):
+            assert "on one another" in message
+            seen[0] += 1
+        elif x != y and set(x) & set(y):
+            assert "itself or lie apart" in message, (T, H, dim, sx, sy, d)
+            seen[1] += 1
+        elif T == 1 or sx[0] == sy[0] or x == y or max(x) < min(y) or max(y) < min(x):
+            assert "positions" in message, (message, T, H, dim, sx, sy, d)
+            seen[2] += 1
+    assert min(seen) > 300, seen
