@@ -293,6 +293,8 @@ __global__ void __launch_bounds__(256) read_kernel(ReadArgs a) {
         }
     } else if (rows_ok && length_ok && length == 0) {
         why = 0;  // an idle slot reads as zeros
+    } else if (a.batch.starts && (row < a.batch.starts[0] || row >= a.batch.starts[a.batch.seqs])) {
+        why = 0;  // and so does a row of no sequence
     }
     if (page < 0 && why && lane == 0) atomicOr(a.status, why);
     // 32 bytes of output (a whole sector) a lane: consecutive lanes along a head, then the heads

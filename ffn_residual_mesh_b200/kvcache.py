@@ -204,7 +204,8 @@ class PagedKvCache:
 
     def read(self, layer: int, tables, lengths, starts, rows: int, dtype=None, stream=None):
         """The last tokens of each sequence back from the cache: k and v [rows, kv_heads,
-        head_dim] (code * scale), float32 unless ``dtype``. ``starts`` says how many of each."""
+        head_dim] (code * scale), float32 unless ``dtype``. ``starts`` says how many of each; rows outside
+        them are zeros."""
         import torch
         types = {None: N.F32, torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
         if dtype not in types:

@@ -336,13 +336,14 @@ int ffnrm_kv_destroy(ffnrm_kv *kv);
  * rint(q * (s_old / s)), new ones rint(x / s). Non-finite values make the scale NaN. With
  * `table` the keys are rotated at their positions first, and with q, q_out as well the
  * queries [rows][q_heads][head_dim] (q_out is q or lies apart from it, and apart from k and v; rows of
- * idle slots become zeros). */
+ * idle slots and of no sequence become zeros). */
 int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, const ffnrm_rows *k,
                     const ffnrm_rows *v, const ffnrm_rows *q, const ffnrm_rows *q_out, int q_heads, const float *table,
                     int rotary_dim, int max_positions, int flags, void *stream);
 
 /* The batch's rows back from the cache: k, v [rows][kv_heads][head_dim] contiguous and
- * 32-byte aligned, code * scale in `dtype`. Idle slots read as zeros. */
+ * 32-byte aligned, code * scale in `dtype`. Idle slots and rows before starts[0] or past starts[seqs] read
+ * as zeros. */
 int ffnrm_kv_read(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtype, void *k, void *v, void *stream);
 
 /* Attention of a step's queries q [rows][q_heads][head_dim] (f16 or bf16; q_heads a multiple

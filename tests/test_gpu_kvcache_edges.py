@@ -265,3 +265,34 @@ def test_in_place_and_in_a_packed_row(cuda, new):
     pos = torch.arange(T, device=cuda).int()
     rotary(x[:, :H], pos, table, out=x[:, H:2 * H])
     assert torch.equal(x[:, H:2 * H], rotary(packed[:, :H], pos, table)) and torch.equal(x[:, 2 * H:], packed[:, 2 * H:])
+
+# ---------------------------------------------------------------------------------- rows of no sequence
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_read_pads_with_zeros(cuda, dtype):
+    """Rows before starts[0] and from starts[seqs] on read as zeros, as they do in append and attend."""
+    import torch
+    cache = make_cache(cuda, 4, 2, 64, 16)
+    tables, lengths = ints([[0, 1], [2, 3]], cuda), ints([20, 9], cuda)
+    kind = {"f16": torch.float16, "f32": torch.float32}[dtype]
+    want = cache.read(0, tables, lengths, ints([0, 3, 5], cuda), 5, dtype=kind)
+    got = cache.read(0, tables, lengths, ints([2, 5, 7], cuda), 11, dtype=kind)
+    cache.check()
+    for g, w in zip(got, want):
+        assert torch.equal(g[2:7], w) and (g[:2] == 0).all() and (g[7:] == 0).all()
+    cache.read(0, tables, ints([20, 1], cuda), ints([0, 3, 5], cuda), 5)  # more rows than tokens: still recorded
+    with pytest.raises(RuntimeError):
+        cache.check()
+
+
+def test_append_pads_with_zeros(cuda):
+    """The same rows in append: no token is taken from them, and their queries become zeros."""
+    import torch
+    tables, lengths = ints([[0, 1], [2, 3]], cuda), ints([20, 9], cuda)
+    table, x = rope_table(32, 64, cuda), torch.randn(11, 2, 64, device=cuda).half()
+    caches = [make_cache(cuda, 4, 2, 64, 16) for _ in range(2)]
+    q = caches[0].append(0, x, x, tables, lengths, starts=ints([2, 5, 7], cuda), rope=table, q=x)
+    want = caches[1].append(0, x[2:7], x[2:7], tables, lengths, starts=ints([0, 3, 5], cuda), rope=table, q=x[2:7])
+    for c in caches:
+        c.check()
+    assert torch.equal(q[2:7], want) and (q[:2] == 0).all() and (q[7:] == 0).all()
+    assert torch.equal(caches[0].k_codes, caches[1].k_codes) and torch.equal(caches[0].v_scale, caches[1].v_scale)
