@@ -478,7 +478,8 @@ int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     const bool has_q = q && q->data;
     if (has_q && !table) return fail(FFNRM_ERR_ARG, "q is only rotated: it needs a rotary table");
     if (has_q && q_heads <= 0) return fail(FFNRM_ERR_ARG, "q_heads=%d must be positive", q_heads);
-    if (batch->rows == 0 || batch->seqs == 0) return FFNRM_OK;
+    if (batch->rows == 0 || (batch->seqs == 0 && !has_q)) return FFNRM_OK;
+    if (batch->seqs == 0) return fail(FFNRM_ERR_ARG, "rows=%d of no sequence", batch->rows);
     if ((rc = check_rows("k", k, dtype)) || (rc = check_rows("v", v, dtype))) return rc;
     if (has_q) {
         if ((rc = check_rows("q_out", q_out, dtype)) || (rc = check_rows("q", q, dtype))) return rc;
@@ -524,7 +525,8 @@ int ffnrm_kv_read(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dtyp
     int rc = check_kv(kv, layer);
     if (rc || (rc = check_batch(kv, batch))) return rc;
     if (dtype < FFNRM_F16 || dtype > FFNRM_F32) return fail(FFNRM_ERR_ARG, "unknown element type %d", dtype);
-    if (batch->rows == 0 || batch->seqs == 0) return FFNRM_OK;
+    if (batch->rows == 0) return FFNRM_OK;
+    if (batch->seqs == 0) return fail(FFNRM_ERR_ARG, "rows=%d of no sequence", batch->rows);
     if (!k || !v || !aligned(k, 32) || !aligned(v, 32)) return fail(FFNRM_ERR_ARG, "k and v must be 32-byte aligned");
     const ReadArgs a{layer_pool(kv, layer), batch_view(batch), k, v, kv->status};
     DeviceGuard guard(kv->device);

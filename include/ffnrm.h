@@ -321,7 +321,8 @@ typedef struct {
 /* One step's batch, all device memory. tables [seqs][table_width] page ids; lengths [seqs]
  * tokens held, the step's new ones included; starts [seqs + 1] the rows of the new tokens
  * (NULL: one row per sequence, rows = seqs). The j-th of a sequence's n rows stands at
- * position lengths - n + j. A sequence of length 0 is an idle slot. */
+ * position lengths - n + j. A sequence of length 0 is an idle slot. Rows of a batch without sequences have
+ * no output: they are refused. */
 typedef struct {
     const int32_t *tables, *lengths, *starts;
     int32_t seqs, table_width, rows;

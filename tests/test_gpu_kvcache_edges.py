@@ -296,3 +296,17 @@ def test_append_pads_with_zeros(cuda):
         c.check()
     assert torch.equal(q[2:7], want) and (q[:2] == 0).all() and (q[7:] == 0).all()
     assert torch.equal(caches[0].k_codes, caches[1].k_codes) and torch.equal(caches[0].v_scale, caches[1].v_scale)
+
+
+def test_rows_of_no_sequence_are_refused(cuda):
+    """With no sequence at all there is nothing that the outputs could be."""
+    import torch
+    cache = make_cache(cuda, 4, 2, 64, 16)
+    t0, none, start = torch.empty(0, 3, dtype=torch.int32, device=cuda), ints([], cuda), ints([0], cuda)
+    x = torch.randn(5, 2, 64, device=cuda).half()
+    for call in (lambda: cache.read(0, t0, none, start, 5), lambda: cache.append(0, x, x, t0, none, starts=start, rope=rope_table(8, 64, cuda), q=x),
+                 lambda: cache.attend(0, x, t0, none, starts=start)):
+        with pytest.raises(ValueError):
+            call()
+    cache.append(0, x, x, t0, none, starts=start)  # nothing to write, nothing to return
+    cache.check()
