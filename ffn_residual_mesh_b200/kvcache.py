@@ -16,7 +16,8 @@ The j-th of a sequence's n new tokens stands at position ``lengths - n + j``. A 
 Arguments are torch tensors on the cache's device. Shape and type errors raise
 ``ValueError``; data on the device that a kernel could not use is recorded and raised by
 ``check``. Calls run on the current stream (or ``stream``) without synchronising and can be
-captured in a CUDA graph; calls on one cache must not overlap on the GPU.
+captured in a CUDA graph; calls on one cache must not overlap on the GPU. Only ``rotary`` takes part in
+autograd: the cache's calls serve, and their results require no gradient.
 """
 from __future__ import annotations
 
@@ -111,10 +112,45 @@ class RotaryTable:
         self.flags = N.ROTARY_INTERLEAVED if interleaved else 0
 
 
+_recorded = None
+
+
+def _rotary_function():
+    """The rotation for autograd: linear in x, its gradient is the other direction at the same positions."""
+    global _recorded
+    if _recorded is None:
+        import torch
+
+        class Rotary(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, x, positions, table, inverse, stream):
+                ctx.save_for_backward(positions, table.cos_sin)
+                ctx.interleaved, ctx.inverse = table.interleaved, inverse
+                return rotary(x.detach(), positions, table, inverse=inverse, stream=stream)
+
+            @staticmethod
+            def backward(ctx, grad):
+                positions, cos_sin = ctx.saved_tensors
+                if grad.stride(2) != 1:  # as a sum's gradient
+                    grad = grad.contiguous()
+                table = RotaryTable.from_tensor(cos_sin, ctx.interleaved)
+                return rotary(grad, positions, table, inverse=not ctx.inverse), None, None, None, None
+
+        _recorded = Rotary
+    return _recorded
+
+
 def rotary(x, positions, table: RotaryTable, out=None, inverse: bool = False, stream=None):
     """x [T, heads, dim] with its first ``rotary_dim`` channels rotated at ``positions`` (int32
-    [T]); ``inverse`` applies the transposed rotation, the gradient of the forward one.
-    ``out`` is x or lies apart from it. A position outside the table gives NaN in the rotated channels."""
+    [T]); ``inverse`` applies the transposed rotation, the gradient of the forward one, which autograd
+    uses where x requires it (the table gets none). ``out`` is x or lies apart from it, and is not for
+    tensors that require a gradient. A position outside the table gives NaN in the rotated channels."""
+    if getattr(x, "requires_grad", False) or getattr(out, "requires_grad", False):
+        import torch
+        if torch.is_grad_enabled():
+            if out is not None:
+                raise ValueError("out= takes no part in autograd: x and out must not require a gradient")
+            return _rotary_function().apply(x, positions, table, inverse, stream)
     return (_module or _bind()).rotary(x, positions, table.cos_sin, out, table.flags | (N.ROTARY_INVERSE if inverse else 0), stream)
 
 

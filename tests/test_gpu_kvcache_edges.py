@@ -310,3 +310,73 @@ def test_rows_of_no_sequence_are_refused(cuda):
             call()
     cache.append(0, x, x, t0, none, starts=start)  # nothing to write, nothing to return
     cache.check()
+
+
+# ---------------------------------------------------------------------------------- autograd
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_gradient_through_autograd(cuda, dtype, interleaved, inverse):
+    """The gradient is the other direction's rotation of the output's, bit for bit; also of a sum (an expanded
+    gradient), of a packed row, of one head shared by several, and twice."""
+    import torch
+    from test_gpu_kvcache import types
+    from ffn_residual_mesh_b200.kvcache import rotary
+    kind, table = types()[dtype], rope_table(40, 32, cuda, interleaved)
+    pos = ints([0, 7, 39, 7, 1], cuda)
+    g = torch.Generator(device=cuda).manual_seed(2)
+    x = torch.randn(5, 6, 48, device=cuda, generator=g).to(kind).requires_grad_()
+    w = torch.randn(5, 3, 48, device=cuda, generator=g).to(kind)
+    y = rotary(x[:, 1:4], pos, table, inverse=inverse)
+    assert y.requires_grad and torch.equal(y.detach(), rotary(x.detach()[:, 1:4], pos, table, inverse=inverse))
+    (got,) = torch.autograd.grad(y, x, w)
+    assert torch.equal(got[:, 1:4], rotary(w, pos, table, inverse=not inverse)) and (got[:, 0] == 0).all() and (got[:, 4:] == 0).all()
+    ones = torch.ones_like(w)
+    (got,) = torch.autograd.grad(rotary(x[:, 1:4], pos, table, inverse=inverse).sum(), x)
+    assert torch.equal(got[:, 1:4], rotary(ones, pos, table, inverse=not inverse))
+    shared = torch.randn(5, 1, 48, device=cuda, generator=g).requires_grad_()
+    (got,) = torch.autograd.grad(rotary(shared.expand(5, 3, 48), pos, table, inverse=inverse), shared, w.float())
+    want = rotary(w.float(), pos, table, inverse=not inverse).double().sum(1, keepdim=True)
+    assert ((got.double() - want).abs() <= 3 * 2.0 ** -23 * (1 + want.abs()) * 4).all()
+    v = w.clone().requires_grad_()  # linear in the output's gradient too
+    (first,) = torch.autograd.grad(rotary(x[:, 1:4], pos, table, inverse=inverse), x, v, create_graph=True)
+    (second,) = torch.autograd.grad(first, v, torch.ones_like(first))
+    assert torch.equal(second, rotary(ones, pos, table, inverse=inverse))
+
+
+def test_rotary_gradient_against_differences(cuda):
+    import torch
+    from ffn_residual_mesh_b200.kvcache import rotary
+    table, pos = rope_table(40, 16, cuda), ints([3, 39], cuda)
+    g = torch.Generator(device=cuda).manual_seed(4)
+    x = torch.randn(2, 2, 20, device=cuda, generator=g).requires_grad_()
+
+    def loss(z):  # a smooth function of the rotated values, in 64 bits behind the kernel
+        return (rotary(z, pos, table).double() ** 3).sum()
+
+    (got,) = torch.autograd.grad(loss(x), x)
+    with torch.no_grad():
+        for t, h, d in ((0, 0, 0), (0, 1, 7), (1, 0, 8), (1, 1, 15), (1, 1, 19)):
+            step = torch.zeros_like(x)
+            step[t, h, d] = 2.0 ** -7
+            diff = (loss(x + step) - loss(x - step)).item() / 2.0 ** -6
+            # f32 rounding of values up to 5 (3 y^2 <= 75 of 2^-22 each, over the step) and the cube's third derivative
+            assert abs(diff - got[t, h, d].item()) <= 40 * 75 * 2.0 ** -22 * 64 + 2.0 ** -14 * 4 + 1e-5 * abs(diff)
+
+
+def test_rotary_into_memory_and_autograd(cuda):
+    import torch
+    from ffn_residual_mesh_b200.kvcache import rotary
+    table, pos = rope_table(8, 16, cuda), ints([1, 2], cuda)
+    x = torch.randn(2, 2, 16, device=cuda).requires_grad_()
+    for bad in (dict(out=torch.empty(2, 2, 16, device=cuda)), dict(out=x)):
+        with pytest.raises(ValueError):
+            rotary(x, pos, table, **bad)
+    with pytest.raises(ValueError):
+        rotary(x.detach(), pos, table, out=torch.empty(2, 2, 16, device=cuda, requires_grad=True))
+    with torch.no_grad():
+        y = rotary(x, pos, table)
+        assert not y.requires_grad and torch.equal(rotary(x, pos, table, out=torch.empty_like(y)), y)
+    with torch.inference_mode():
+        z = x.detach().clone()
+        assert torch.equal(rotary(z, pos, table, out=z), y)
