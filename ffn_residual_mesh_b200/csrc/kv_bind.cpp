@@ -105,6 +105,13 @@ void writable(const char *name, const at::Tensor &x) {
         if (x.stride(i) == 0 && x.size(i) > 1) refuse("%s must not be an expanded view", name);
 }
 
+// A caller's tensor has new contents: autograd's saved copies of it are out of date.
+void written(PyObject *o) {
+    if (o == Py_None) return;
+    const at::Tensor &x = THPVariable_Unpack(o);
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+
 int32_t *ints(const char *name, const at::Tensor &x, int device) {
     if (x.scalar_type() != at::kInt || !x.is_contiguous()) refuse("%s must be a contiguous int32 tensor", name);
     on(name, x, device);
@@ -200,6 +207,7 @@ PyObject *rotary(PyObject *const *a) {
     check(ffnrm_rotary(&xr, &yr, dtype, int32_of("T", T), int32_of("heads", heads), int32_of("dim", dim), pos, table.data_ptr<float>(),
                        int32_of("rotary_dim", table.size(1)), int32_of("max_positions", table.size(0)), int(integer(a[4])),
                        stream.ptr));
+    written(a[3]);
     return THPVariable_Wrap(std::move(out));
 }
 
@@ -246,6 +254,7 @@ PyObject *append(PyObject *const *a) {
     check(ffnrm_kv_append(geo.kv, layer, &batch, dtype, &kr, &vr, &qr, &yr, int32_of("heads", heads), table, rot, positions,
                           int(integer(a[8])), stream.ptr));
     if (!out.defined()) Py_RETURN_NONE;
+    written(a[10]);
     return THPVariable_Wrap(std::move(out));
 }
 
@@ -282,6 +291,8 @@ PyObject *attend(PyObject *const *a) {
     if (causal < 0 || PyErr_Occurred()) throw Refused();
     check(ffnrm_kv_attend(geo.kv, int32_of("layer", integer(a[1])), &batch, dtype, &qr, &yr, lse, int32_of("heads", heads), float(scale),
                           causal, int32_of("window", integer(a[10])), stream.ptr));
+    written(a[6]);
+    written(a[7]);
     return THPVariable_Wrap(std::move(out));
 }
 
@@ -317,6 +328,7 @@ PyObject *fork(PyObject *const *a) {
                         int32_of("width", t.size(1)), ints1("parents", parents, n, d), ints1("extra", tensor("extra", a[4]), n, d),
                         int32_of("children", n), ints("out_tables", out, d), int32_of("width", out.size(1)),
                         ints1("out_lengths", lens, n, d), ints1("info", info, 4, d), stream.ptr));
+    for (int i : {5, 6, 7}) written(a[i]);
     return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lens)), THPVariable_Wrap(std::move(info)));
 }
 
@@ -332,6 +344,7 @@ PyObject *compact(PyObject *const *a) {
     check(ffnrm_kv_compact(geo.kv, ints("tables", t, d), ints1("lengths", tensor("lengths", a[2]), t.size(0), d),
                            int32_of("seqs", t.size(0)), int32_of("width", t.size(1)), ints("out_tables", out, d),
                            ints1("info", info, 4, d), stream.ptr));
+    for (int i : {3, 4}) written(a[i]);
     return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(info)));
 }
 

@@ -380,3 +380,38 @@ def test_rotary_into_memory_and_autograd(cuda):
     with torch.inference_mode():
         z = x.detach().clone()
         assert torch.equal(rotary(z, pos, table, out=z), y)
+
+
+def test_outputs_that_are_given_count_as_written(cuda):
+    """Their version moves, so that autograd does not take a saved tensor for what it was."""
+    import torch
+    from ffn_residual_mesh_b200.kvcache import rotary
+    cache, table = make_cache(cuda, 8, 2, 64, 16), rope_table(64, 64, cuda)
+    tables, lengths = ints([[0, 1], [2, 3]], cuda), ints([20, 9], cuda)
+    q, k = torch.randn(2, 4, 64, device=cuda).half(), torch.randn(2, 2, 64, device=cuda).half()
+    out, lse = torch.empty_like(q), torch.empty(2, 4, device=cuda)
+    t2, l2, info = torch.empty_like(tables), torch.empty_like(lengths), ints([0] * 4, cuda)
+    two = ints([0, 1], cuda)
+    for call, given in ((lambda: rotary(q, two, table, out=out), (out,)),
+                        (lambda: cache.append(0, k, k, tables, lengths, rope=table, q=q, q_out=out), (out,)),
+                        (lambda: cache.attend(0, q, tables, lengths, out=out, lse=lse), (out, lse)),
+                        (lambda: cache.fork(tables, lengths, two, two, out_tables=t2, out_lengths=l2, info=info), (t2, l2, info)),
+                        (lambda: cache.compact(tables, lengths, out_tables=t2, info=info), (t2, info))):
+        before = [x._version for x in (*given, q, k, tables, lengths)]
+        call()
+        after = [x._version for x in (*given, q, k, tables, lengths)]
+        assert [b > a for a, b in zip(before, after)] == [True] * len(given) + [False] * 4
+    scale = torch.ones_like(q, requires_grad=True)
+    y = scale * out  # saves out
+    cache.attend(0, q, tables, lengths, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        cache.attend(0, q, tables, lengths, out=torch.empty_like(q))
+        cache.attend(0, q, tables, lengths, out=out)
+    inside = None
+    with torch.inference_mode():
+        inside = torch.empty_like(q)
+    cache.attend(0, q, tables, lengths, out=inside)
+    assert torch.equal(inside, out)
+    cache.check()
