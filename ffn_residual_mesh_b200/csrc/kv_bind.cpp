@@ -13,6 +13,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <exception>
+#include <initializer_list>
 
 #include "ffnrm.h"
 
@@ -127,10 +128,18 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, int device) {
 }
 
 // The call's stream: the current one, or the one that is given, which is then current for the call, so
-// that a new output's memory belongs to the stream that writes it.
+// that a new output's memory belongs to the stream that writes it. `keep` holds the caller's tensors, which
+// belong to other streams, until the call's work on it is done, should the caller drop them before.
 struct Stream {
     c10::OptionalStreamGuard guard;
     void *ptr;
+    bool other = false;  // not the current stream
+    void keep(std::initializer_list<PyObject *> tensors) const {
+        if (!other) return;
+        const c10::Stream stream = *guard.current_stream();
+        for (PyObject *o : tensors)
+            if (THPVariable_Check(o)) THPVariable_Unpack(o).record_stream(stream);
+    }
     Stream(PyObject *o, int device) {
         const c10::DeviceIndex d(device);
         if (o == Py_None) {
@@ -146,6 +155,7 @@ struct Stream {
             Py_DECREF(v);
         }
         if (!ptr && PyErr_Occurred()) throw Refused();
+        other = ptr != c10::cuda::getCurrentCUDAStream(d).stream();
         guard.reset_stream(ptr ? c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(ptr), d)
                                : c10::cuda::getDefaultCUDAStream(d));
     }
@@ -207,6 +217,7 @@ PyObject *rotary(PyObject *const *a) {
     check(ffnrm_rotary(&xr, &yr, dtype, int32_of("T", T), int32_of("heads", heads), int32_of("dim", dim), pos, table.data_ptr<float>(),
                        int32_of("rotary_dim", table.size(1)), int32_of("max_positions", table.size(0)), int(integer(a[4])),
                        stream.ptr));
+    stream.keep({a[0], a[1], a[2], a[3]});
     written(a[3]);
     return THPVariable_Wrap(std::move(out));
 }
@@ -253,6 +264,7 @@ PyObject *append(PyObject *const *a) {
     const int layer = int32_of("layer", integer(a[1]));
     check(ffnrm_kv_append(geo.kv, layer, &batch, dtype, &kr, &vr, &qr, &yr, int32_of("heads", heads), table, rot, positions,
                           int(integer(a[8])), stream.ptr));
+    stream.keep({a[2], a[3], a[4], a[5], a[6], a[7], a[9], a[10]});
     if (!out.defined()) Py_RETURN_NONE;
     written(a[10]);
     return THPVariable_Wrap(std::move(out));
@@ -291,6 +303,7 @@ PyObject *attend(PyObject *const *a) {
     if (causal < 0 || PyErr_Occurred()) throw Refused();
     check(ffnrm_kv_attend(geo.kv, int32_of("layer", integer(a[1])), &batch, dtype, &qr, &yr, lse, int32_of("heads", heads), float(scale),
                           causal, int32_of("window", integer(a[10])), stream.ptr));
+    stream.keep({a[2], a[3], a[4], a[5], a[6], a[7]});
     written(a[6]);
     written(a[7]);
     return THPVariable_Wrap(std::move(out));
@@ -306,6 +319,7 @@ PyObject *read(PyObject *const *a) {
     const ffnrm_kv_batch batch = batch_of(a[2], a[3], a[4], rows, geo.device);
     at::Tensor k = empty({rows, geo.heads, geo.dim}, type, geo.device), v = empty({rows, geo.heads, geo.dim}, type, geo.device);
     check(ffnrm_kv_read(geo.kv, int32_of("layer", integer(a[1])), &batch, int(dtype), k.data_ptr(), v.data_ptr(), stream.ptr));
+    stream.keep({a[2], a[3], a[4]});
     return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
 }
 
@@ -328,6 +342,7 @@ PyObject *fork(PyObject *const *a) {
                         int32_of("width", t.size(1)), ints1("parents", parents, n, d), ints1("extra", tensor("extra", a[4]), n, d),
                         int32_of("children", n), ints("out_tables", out, d), int32_of("width", out.size(1)),
                         ints1("out_lengths", lens, n, d), ints1("info", info, 4, d), stream.ptr));
+    stream.keep({a[1], a[2], a[3], a[4], a[5], a[6], a[7]});
     for (int i : {5, 6, 7}) written(a[i]);
     return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lens)), THPVariable_Wrap(std::move(info)));
 }
@@ -344,6 +359,7 @@ PyObject *compact(PyObject *const *a) {
     check(ffnrm_kv_compact(geo.kv, ints("tables", t, d), ints1("lengths", tensor("lengths", a[2]), t.size(0), d),
                            int32_of("seqs", t.size(0)), int32_of("width", t.size(1)), ints("out_tables", out, d),
                            ints1("info", info, 4, d), stream.ptr));
+    stream.keep({a[1], a[2], a[3], a[4]});
     for (int i : {3, 4}) written(a[i]);
     return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(info)));
 }
@@ -356,6 +372,7 @@ PyObject *copy_pages(PyObject *const *a) {
     if (src.dim() != 1) refuse("src must have shape (n,)");
     check(ffnrm_kv_copy_pages(geo.kv, ints("src", src, geo.device), ints1("dst", tensor("dst", a[2]), src.size(0), geo.device),
                               int32_of("n", src.size(0)), stream.ptr));
+    stream.keep({a[1], a[2]});
     Py_RETURN_NONE;
 }
 

@@ -16,7 +16,9 @@ The j-th of a sequence's n new tokens stands at position ``lengths - n + j``. A 
 Arguments are torch tensors on the cache's device. Shape and type errors raise
 ``ValueError``; data on the device that a kernel could not use is recorded and raised by
 ``check``. Calls run on the current stream (or ``stream``) without synchronising and can be
-captured in a CUDA graph; calls on one cache must not overlap on the GPU. Only ``rotary`` takes part in
+captured in a CUDA graph; calls on one cache must not overlap on the GPU. With a ``stream`` that is not
+the current one the caller orders it behind what wrote the arguments (they may be dropped as soon as the
+call returns); new outputs belong to that stream. Only ``rotary`` takes part in
 autograd: the cache's calls serve, and their results require no gradient.
 """
 from __future__ import annotations

@@ -415,3 +415,50 @@ def test_outputs_that_are_given_count_as_written(cuda):
     cache.attend(0, q, tables, lengths, out=inside)
     assert torch.equal(inside, out)
     cache.check()
+
+
+# ---------------------------------------------------------------------------------- another stream
+def test_arguments_may_be_dropped_while_another_stream_works(cuda):
+    """The side stream is kept busy for some 50 ms; what the calls read there is dropped on the current one and
+    its memory asked for again."""
+    import torch
+    from ffn_residual_mesh_b200.kvcache import RotaryTable, rotary
+    H, G, D, T = 4, 8, 128, 64
+    rows = [[2 * i, 2 * i + 1] for i in range(T)]
+    lengths = [3 + i % 29 for i in range(T)]
+
+    def work(stream, drop):
+        """q's and k's rotation, append, attend, read, fork, compact; every argument made here."""
+        cache = make_cache(cuda, 2 * T + 8, H, D, 16, max_seqs=T, seed=1)
+        g = torch.Generator(device=cuda).manual_seed(3)
+        q, k = (torch.randn(T, n, D, device=cuda, generator=g).half() for n in (H * G, H))
+        t, n, pos = ints(rows, cuda), ints(lengths, cuda), ints(lengths, cuda)
+        table, starts = rope_table(64, D, cuda), ints(list(range(T + 1)), cuda)
+        parents, extra = ints(list(range(T))[::-1], cuda), ints([1] * T, cuda)
+        lse = torch.empty(T, H * G, device=cuda)
+        if stream is not None:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                torch.cuda._sleep(100_000_000)
+        r = rotary(q, pos, table, stream=stream)
+        a = cache.append(0, k, k, t, n, starts=starts, rope=table, q=q, stream=stream)
+        o = cache.attend(0, q, t, n, starts=starts, lse=lse, stream=stream)
+        back = cache.read(0, t, n, starts, T, stream=stream)
+        f = cache.fork(t, n, parents, extra, stream=stream)
+        c = cache.compact(t, n, stream=stream)
+        if drop:
+            size = [x.shape for x in (q, k, t, n, pos, starts, parents, table.cos_sin)]
+            kind = [x.dtype for x in (q, k, t, n, pos, starts, parents, table.cos_sin)]
+            del q, k, t, n, pos, starts, parents, extra, table
+            again = [torch.full(s, 3, dtype=d, device=cuda) for s, d in zip(size, kind) for _ in range(3)]
+            torch.cuda.current_stream().synchronize()
+            del again
+        if stream is not None:
+            stream.synchronize()
+        cache.check(stream)
+        return [r, a, o, lse, *back, *f, *c, cache.k_codes, cache.k_scale, cache.v_codes]
+
+    want = work(None, False)
+    got = work(torch.cuda.Stream(), True)
+    for i, (x, y) in enumerate(zip(got, want)):
+        assert torch.equal(x, y), i
