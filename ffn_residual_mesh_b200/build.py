@@ -13,6 +13,7 @@ import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -63,9 +64,40 @@ def included(source: Path) -> list[Path]:
     return found
 
 
-# Python binding of the paged cache's calls (torch tensors in, C ABI out).
+# Python binding of the paged cache's calls (torch tensors in, C ABI out). It belongs to one torch and one Python, which
+# the stamp beside it names; the library and the runners need neither.
 BIND_SOURCE = CSRC / "kv_bind.cpp"
 BIND = LIB_DIR / "ffnrm_kv_bind.so"
+BIND_STAMP = LIB_DIR / "ffnrm_kv_bind.stamp"
+
+
+def bind_versions() -> str | None:
+    """Versions that the binding is built against; None without a torch."""
+    try:
+        return f"torch {metadata.version('torch')}, {sys.implementation.cache_tag}"
+    except metadata.PackageNotFoundError:
+        return None
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path | None:
+    """The binding, or None (and a message) where there is no torch with CUDA; kvcache then says that it is missing."""
+    versions = bind_versions()
+    if versions is None:
+        print("no torch: the Python binding of the paged cache is not built", file=sys.stderr)
+        return None
+    same = BIND_STAMP.exists() and BIND_STAMP.read_text() == versions
+    if not force and same and not stale(BIND, [BIND_SOURCE, ROOT / "include" / "ffnrm.h"]):
+        return BIND
+    import torch
+    if torch.version.cuda is None:
+        print("torch without CUDA: the Python binding of the paged cache is not built", file=sys.stderr)
+        return None
+    cmd = bind_command()
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    BIND_STAMP.write_text(versions)
+    return BIND
 
 
 def bind_command() -> list[str]:
@@ -128,13 +160,9 @@ def build(force: bool = False, verbose: bool = False, runners: bool = True) -> P
             for done in pool.map(subprocess.run, todo):
                 done.check_returncode()
         subprocess.run(link_command(), check=True)
-    if force or stale(BIND, [BIND_SOURCE, ROOT / "include" / "ffnrm.h"]):
-        cmd = bind_command()
-        if verbose:
-            print(" ".join(cmd), file=sys.stderr)
-        subprocess.run(cmd, check=True)
     if runners:
         build_runners(force, verbose)
+    build_binding(force, verbose)
     return LIB
 
 
