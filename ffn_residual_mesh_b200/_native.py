@@ -97,11 +97,6 @@ class KvBatch(ctypes.Structure):
                 ("table_width", c_int32), ("rows", c_int32)]
 
 
-class KvBatch(ctypes.Structure):
-    _fields_ = [("tables", c_void_p), ("lengths", c_void_p), ("starts", c_void_p), ("seqs", c_int32),
-                ("table_width", c_int32), ("rows", c_int32)]
-
-
 class Rows(ctypes.Structure):
     _fields_ = [("data", c_void_p), ("token_stride", c_int64), ("head_stride", c_int64)]
 
