@@ -18,6 +18,8 @@
 namespace ffnrm::kv {
 
 constexpr float kLeastScale = 0x1p-64f, kZeroScale = 0x1p-40f;
+// 1 / sv; the fast division gives 0 from 2^126 on, so it works on a quarter.
+__device__ __forceinline__ float inverse_scale(float sv) { return 0.25f * __fdividef(1.f, 0.25f * sv); }
 // Whether a block's values count as zero (a NaN or negative scale does not).
 __device__ __forceinline__ bool zero_block(float sv) { return fabsf(sv) < kLeastScale; }
 

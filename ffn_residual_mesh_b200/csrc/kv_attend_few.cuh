@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(W * 32, few_blocks<D, NT, W>()) attend_few_ker
                         for (int c = 0; c < VB / 4; ++c) xv[r][c] = 0;
                 }
             }
-            const float vlog = lg2(vs), vinv = vs == vs ? __fdividef(1.f, vs) : 0.f;
+            const float vlog = lg2(vs), vinv = vs == vs ? inverse_scale(vs) : 0.f;
             const bool whole = key + 16 <= all_hi && key >= all_lo;
             bool raise = false;
 #pragma unroll

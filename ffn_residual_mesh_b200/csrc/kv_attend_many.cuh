@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(Many<D>::THREADS, 1) attend_many_kernel(ManyAr
             // a NaN value scale reaches the rows that see it through its logarithm
             if (v && lane < RUNS)
                 sm_scale[st * C::CHUNKS + w * RUNS + lane] =
-                    make_float4(sc.x, sc.y == kNoPage ? ninf : lg2(sc.y), sc.y > 0.f ? __fdividef(1.f, sc.y) : 0.f, 0.f);
+                    make_float4(sc.x, sc.y == kNoPage ? ninf : lg2(sc.y), sc.y > 0.f ? inverse_scale(sc.y) : 0.f, 0.f);
             store((v ? sm_v : sm_k) + st * C::KV_BYTES, r);
             fence_proxy_async_smem();
             __syncwarp();

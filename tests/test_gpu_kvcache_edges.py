@@ -462,3 +462,14 @@ def test_arguments_may_be_dropped_while_another_stream_works(cuda):
     got = work(torch.cuda.Stream(), True)
     for i, (x, y) in enumerate(zip(got, want)):
         assert torch.equal(x, y), i
+
+
+@pytest.mark.parametrize("value", [1e18, 1e36, 9e37, 3e38])
+def test_value_scales_up_to_the_largest(cuda, value):
+    """Codes of -1, 0 and 1 under scales up to f32's largest: also those whose reciprocal is a subnormal."""
+    def large(cache, rows, q):
+        cache.v_codes.clamp_(-1, 1)
+        cache.v_scale.fill_(value)
+    check_attend(cuda, [1, 1], [300, 17], 2, 4, 128, 32, "bf16", seed=1, tamper=large, with_starts=False)
+    check_attend(cuda, [300, 20], [300, 600], 2, 4, 128, 32, "bf16", seed=1, tamper=large)
+    check_attend(cuda, [200], [256], 1, 4, 256, 64, "bf16", seed=1, tamper=large, causal=False)
