@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/core/StreamGuard.h>
@@ -193,11 +194,15 @@ PyObject *guarded(PyObject *const *args, Py_ssize_t n, Py_ssize_t want) {
     }
 }
 
-// x, positions, cos_sin, out or None, flags, stream
+// x, positions, cos_sin, out or None, flags, stream. None (and nothing done) for an x that autograd follows.
 PyObject *rotary(PyObject *const *a) {
     const at::Tensor &x = tensor("x", a[0]), &table = tensor("table", a[2]);
     if (x.dim() != 3) refuse("x must have shape (T, heads, dim)");
     if (!x.is_cuda()) refuse("x must be on a CUDA device");
+    if (at::GradMode::is_enabled() && (x.requires_grad() || (a[3] != Py_None && tensor("out", a[3]).requires_grad()))) {
+        if (a[3] != Py_None) refuse("out= takes no part in autograd: x and out must not require a gradient");
+        Py_RETURN_NONE;
+    }
     const int device = x.get_device(), dtype = dtype_of(x);
     const Stream stream(a[5], device);
     const int64_t T = x.size(0), heads = x.size(1), dim = x.size(2);

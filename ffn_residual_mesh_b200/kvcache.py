@@ -147,13 +147,8 @@ def rotary(x, positions, table: RotaryTable, out=None, inverse: bool = False, st
     [T]); ``inverse`` applies the transposed rotation, the gradient of the forward one, which autograd
     uses where x requires it (the table gets none). ``out`` is x or lies apart from it, and is not for
     tensors that require a gradient. A position outside the table gives NaN in the rotated channels."""
-    if getattr(x, "requires_grad", False) or getattr(out, "requires_grad", False):
-        import torch
-        if torch.is_grad_enabled():
-            if out is not None:
-                raise ValueError("out= takes no part in autograd: x and out must not require a gradient")
-            return _rotary_function().apply(x, positions, table, inverse, stream)
-    return (_module or _bind()).rotary(x, positions, table.cos_sin, out, table.flags | (N.ROTARY_INVERSE if inverse else 0), stream)
+    y = (_module or _bind()).rotary(x, positions, table.cos_sin, out, table.flags | (N.ROTARY_INVERSE if inverse else 0), stream)
+    return _rotary_function().apply(x, positions, table, inverse, stream) if y is None else y
 
 
 class PagedKvCache:
