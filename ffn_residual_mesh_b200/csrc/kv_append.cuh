@@ -12,7 +12,8 @@
 //
 // Bound by issue slots (rotation, two looks at a value, the quotient) and by the chain of dependent loads
 // before the values: 11.5k tokens of 8 kv heads x 128 with 32 heads of q, bf16: 65 us (3.7 TB/s);
-// 64 single tokens: 8.2 us. Reading them back in f32: 28 us (4.3 TB/s).
+// 64 single tokens: 8.2 us. Reading them back in f32: 28 us (4.3 TB/s). The half layout's 16-byte path spills some of its
+// 64 registers (append and read together, times their floor: 1.73 in half layout, 1.58 interleaved).
 #pragma once
 
 #include "kv_common.cuh"

@@ -13,9 +13,12 @@
 // The running maximum moves only when a score passes it by 2^8 (p stays below 2^15 in f16 with
 // the 2^7 offset), which a vote per 16 keys decides.
 //
-// Bound by the issue slots of the conversion: 411 instructions for 16 keys x 128 channels, half of them
+// Bound by the issue slots of the conversion: 418 instructions for 16 keys x 128 channels, half of them
 // widening int8 to f16, against HBM at 4.6 TB/s (24 contexts of up to 32k tokens, 8 kv heads x 128,
-// 64 query heads: 358 MB in 75-79 us, 70% of the measured copy rate; one context of 131072: 67 us).
+// 64 query heads: 358 MB in 76-79 us, 70% of the measured copy rate; one context of 131072: 67 us). Short contexts
+// pay for the item itself, whose eight warps join through shared memory however few keys they had (39 contexts of
+// up to 418 keys, 16 x 16 heads: 37 us for 3.5 us of bytes). At head dim 256 with 9 to 16 rows the kernel has 255
+// registers, spills some and runs one block an SM (22 contexts of up to 846 keys: 57 us for 8.4 us of bytes).
 //
 // Work split: all (sequence, kv head, row tile) items, cut into units of 16 W keys, are laid on a
 // line; each block takes an equal stretch of it. An item cut between blocks leaves partial
@@ -93,7 +96,10 @@ struct FewArgs {
 
 // The stretch of a sequence that its rows see, in units of UK keys, and its row tiles. On the line an item
 // takes kFewItem units more, about what its queries, first loads and output cost beside the keys
-// (without them a block with 18 short items ran three times as long as one with 50 units of one).
+// (without them a block with 18 short items ran three times as long as one with 50 units of one). Extra units of
+// 1 / 3 / 6 / 10, us: 24 contexts of up to 32k tokens at head dim 128 85 / 77 / 79 / 82, 64 91 / 84 / 86 / 88, 256 103 / 92 / 97 /
+// 100, in the 16-row variant 88 / 73 / 74 / 78; 256 contexts of up to 2048 100 / 89 / 101 / 113; 39 of up to 418 39 / 37 / 41 /
+// 41; 22 of up to 846 at head dim 256 61 / 57 / 61 / 64; 16 x 5 tokens 59 / 42 / 45 / 51.
 constexpr int kFewItem = 3;
 struct SeqWork {
     int first, n, length, unit0, units, tiles;

@@ -17,7 +17,9 @@
 // Per 128 keys and 256 rows the products need 2048 cycles and the exponentials left to the MUFU 1792; the
 // loop takes some 4200, the chain S - softmax - P - products with its hand-overs (116 cycles each) being
 // longer than either. Measured: 8192-token prompt, 32/8 heads x 128, causal: 580-591 us, 930-948
-// TFLOP/s (57% of the measured GEMM burst); 4096 tokens at head dim 256: 350-357 us.
+// TFLOP/s (57% of the measured GEMM burst); 4096 tokens at head dim 256: 345-357 us. A block has its set-up, query tile,
+// first conversion and output to itself (one block an SM): with four key tiles to a block they weigh most (a prompt
+// of 1073 tokens, 16 x 16 heads: 167 us for 46 us of products).
 #pragma once
 
 #include <type_traits>

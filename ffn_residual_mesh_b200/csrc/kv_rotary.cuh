@@ -103,7 +103,7 @@ __device__ __forceinline__ void rotate_unit(const T *x, T *y, int64_t x_head, in
 }
 
 // One thread per unit of HEADS head rows. Bound by reading and writing x once (16384 x 32 x 128 bf16, half
-// of it rotated: 53 us, 5.1 TB/s, 78% of the measured copy rate; one head to a thread 74 us): several rows under way per
+// of it rotated: interleaved 53 us, 5.1 TB/s, 78% of the measured copy rate, one head to a thread 74 us; half layout 66 us): several rows under way per
 // thread keep enough bytes in flight, and a table row is read once for HEADS heads.
 template <typename T, bool INTERLEAVED, int VEC, int HEADS>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a, float sign) {

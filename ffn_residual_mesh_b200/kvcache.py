@@ -2,7 +2,8 @@
 8-bit paged cache (append, attend, read, fork, compact) over the C ABI.
 
 A cache holds K and V as int8 codes in pages of ``page_tokens`` tokens, with one f32 scale
-for each page and head (value = code * scale). A step works on a batch of sequences given by
+for each page and head (value = code * scale; scales are finite and not negative, NaN marks a block that
+took a non-finite value). A step works on a batch of sequences given by
 three int32 device tensors:
 
 * ``tables``  [seqs, width]  page ids of each sequence in order;
