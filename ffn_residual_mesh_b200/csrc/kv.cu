@@ -60,10 +60,10 @@ bool share_bytes(const void *a, size_t na, const void *b, size_t nb) {
 }
 size_t type_size(int dtype) { return dtype == FFNRM_F32 ? 4 : 2; }
 
-// Whether a row block can be read in 16-byte accesses.
-bool wide(const ffnrm_rows &r, int dtype) {
+// Whether a row block can be read in 16-byte accesses (a single token's or head's stride is never used).
+bool wide(const ffnrm_rows &r, int dtype, int tokens, int heads) {
     const int64_t n = 16 / int64_t(type_size(dtype));
-    return aligned(r.data, 16) && r.token_stride % n == 0 && r.head_stride % n == 0;
+    return aligned(r.data, 16) && (tokens == 1 || r.token_stride % n == 0) && (heads == 1 || r.head_stride % n == 0);
 }
 
 int check_rows(const char *name, const ffnrm_rows *r, int dtype) {
@@ -375,7 +375,7 @@ int ffnrm_rotary(const ffnrm_rows *x, const ffnrm_rows *y, int dtype, int tokens
     if (int64_t(tokens) * heads * head_dim / 256 > 0x7fffffff) return fail(FFNRM_ERR_ARG, "tokens=%d are too many for one call", tokens);
     const RotaryArgs a{x->data, y->data, positions, table, x->token_stride, x->head_stride, y->token_stride, y->head_stride,
                        tokens, heads, head_dim, rotary_dim, max_positions};
-    const bool vec = wide(*x, dtype) && wide(*y, dtype), inter = flags & FFNRM_ROTARY_INTERLEAVED;
+    const bool vec = wide(*x, dtype, tokens, heads) && wide(*y, dtype, tokens, heads), inter = flags & FFNRM_ROTARY_INTERLEAVED;
     const float sign = flags & FFNRM_ROTARY_INVERSE ? -1.f : 1.f;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == FFNRM_F16)
@@ -490,7 +490,9 @@ int ffnrm_kv_append(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     }
     const bool inter = flags & FFNRM_ROTARY_INTERLEAVED;
     const int N = 16 / int(type_size(dtype));
-    const bool vec = wide(*k, dtype) && wide(*v, dtype) && (!has_q || (wide(*q, dtype) && wide(*q_out, dtype))) &&
+    const int T = batch->rows, H = kv->cfg.kv_heads;
+    const bool vec = wide(*k, dtype, T, H) && wide(*v, dtype, T, H) &&
+                     (!has_q || (wide(*q, dtype, T, q_heads) && wide(*q_out, dtype, T, q_heads))) &&
                      (!table || rotary_fits(inter, 8, D, rotary_dim, table));
     AppendArgs a{};
     a.pool = layer_pool(kv, layer);
@@ -553,7 +555,7 @@ int ffnrm_kv_attend(ffnrm_kv *kv, int layer, const ffnrm_kv_batch *batch, int dt
     if (batch->rows == 0) return FFNRM_OK;
     if (batch->seqs == 0) return fail(FFNRM_ERR_ARG, "rows=%d of no sequence", batch->rows);
     if ((rc = check_rows("q", q, dtype)) || (rc = check_rows("out", out, dtype))) return rc;
-    if (!wide(*q, dtype) || !wide(*out, dtype))
+    if (!wide(*q, dtype, batch->rows, q_heads) || !wide(*out, dtype, batch->rows, q_heads))
         return fail(FFNRM_ERR_ARG, "q and out rows must be 16-byte aligned");
     if (!aligned(lse, 4)) return fail(FFNRM_ERR_ARG, "lse must be 4-byte aligned");
     const RowPair pair{batch->rows, q_heads, q_heads, kv->cfg.head_dim, type_size(dtype)};

@@ -473,3 +473,24 @@ def test_value_scales_up_to_the_largest(cuda, value):
     check_attend(cuda, [1, 1], [300, 17], 2, 4, 128, 32, "bf16", seed=1, tamper=large, with_starts=False)
     check_attend(cuda, [300, 20], [300, 600], 2, 4, 128, 32, "bf16", seed=1, tamper=large)
     check_attend(cuda, [200], [256], 1, 4, 256, 64, "bf16", seed=1, tamper=large, causal=False)
+
+
+# ---------------------------------------------------------------------------------- strides that count for nothing
+def test_strides_of_single_rows_and_heads_do_not_matter(cuda):
+    """One token or one head: its stride is never used, so it may be anything."""
+    import torch
+    from ffn_residual_mesh_b200.kvcache import rotary
+    cache, table = make_cache(cuda, 4, 1, 64, 16), rope_table(64, 64, cuda)
+    flat = torch.randn(4096, device=cuda).half()
+    tables, one, two = ints([[0, 1]], cuda), ints([20], cuda), ints([[0, 1], [2, 3]], cuda)
+    q = flat[:4 * 64].view(1, 4, 64)
+    odd = flat.as_strided((1, 4, 64), (301, 64, 1))
+    assert torch.equal(cache.attend(0, odd, tables, one), cache.attend(0, q, tables, one))
+    out = torch.zeros(4096, device=cuda).half().as_strided((1, 4, 64), (333, 64, 1))
+    assert torch.equal(cache.attend(0, q, tables, one, out=out), cache.attend(0, q, tables, one))
+    tall = flat.as_strided((2, 1, 64), (64, 37, 1))
+    lengths = ints([20, 9], cuda)
+    assert torch.equal(cache.attend(0, tall, two, lengths), cache.attend(0, tall.contiguous(), two, lengths))
+    z = flat.clone().as_strided((1, 4, 64), (7, 64, 1))
+    assert torch.equal(rotary(z, one, table, out=z.as_strided((1, 4, 64), (99, 64, 1))), rotary(q, one, table))
+    cache.check()
