@@ -494,3 +494,25 @@ def test_strides_of_single_rows_and_heads_do_not_matter(cuda):
     z = flat.clone().as_strided((1, 4, 64), (7, 64, 1))
     assert torch.equal(rotary(z, one, table, out=z.as_strided((1, 4, 64), (99, 64, 1))), rotary(q, one, table))
     cache.check()
+
+
+def test_fork_and_compact_of_the_largest_pool_and_batch(cuda):
+    """2^20 pages and 4096 sequences: the most shared memory that the table kernels take."""
+    import numpy as np
+    import kv_reference as ref
+    rng, P, n, pages, width = np.random.default_rng(3), 16, 4096, 1 << 20, 4
+    lengths = rng.integers(0, 40, n).tolist()
+    ids, at, rows = rng.permutation(pages), 0, []
+    for x in lengths:
+        k = -(-x // P)
+        rows.append([*ids[at:at + k].tolist(), *[-1] * (width - k)])
+        at += k
+    cache = make_cache(cuda, pages, 1, 64, P, max_seqs=n)
+    parents, extra = rng.integers(-1, n, n).tolist(), rng.integers(0, 20, n).tolist()
+    tables, lens, info = cache.fork(ints(rows, cuda), ints(lengths, cuda), ints(parents, cuda), ints(extra, cuda))
+    packed, count = cache.compact(tables, lens)
+    cache.check()
+    want, want_len, copies = ref.fork(rows, lengths, parents, extra, pages, P, width)
+    assert tables.tolist() == want and lens.tolist() == want_len and info[2] == len(copies)
+    want, move = ref.compact(want, want_len, P)
+    assert packed.tolist() == want and count[2] == len(move)
